@@ -274,6 +274,7 @@ class PrefillArgs(ct.Structure):
         ("h_kv", ct.c_int), ("n_q_groups", ct.c_int), ("n_q", ct.c_int), ("n_kv", ct.c_int),
         ("head_dim", ct.c_int), ("dtype", ct.c_int), ("causal", ct.c_int), ("sm_scale", ct.c_float),
         ("n_split", ct.c_int), ("workspace", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+        ("window", ct.c_int), ("sinks", ct.c_int),
     ]
 
 

@@ -39,6 +39,7 @@ SOURCES = {
     "k2b_general.hip": ["-ffp-contract=off"],
     "fp16_decode.hip": ["-ffp-contract=fast"],
     "flash_prefill.hip": ["-ffp-contract=fast"],
+    "prefill_rows.hip": ["-ffp-contract=fast"],
 }
 
 

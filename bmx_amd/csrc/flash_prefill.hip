@@ -27,9 +27,19 @@
 // With one key split per row tile the workgroup writes the normalized rows;
 // with several it writes (O, m, l) partials that prefill_combine_kernel
 // merges by their softmax weights.
+//
+// prefill_kernel<DT, true>: a sliding window with sinks.  The row tile walks
+// the tiles that some row of it sees, the sinks' tiles and then the band's
+// (TileList), and masks those that cross an edge of the band, of the sinks or
+// of the keys.  A hidden key weighs 0, but 0 times an infinite or NaN value is
+// NaN: a masked tile's values are looked over as they are staged, and a tile
+// that holds one goes through a loop that takes only the keys a row sees
+// (values hidden from every row, such as evicted rows of a cache, may hold
+// anything).
 
 #include "bmx_prefill.h"
 #include "k2b_common.h"
+#include "prefill_rows.h"
 
 #include <hip/hip_runtime.h>
 
@@ -64,7 +74,32 @@ struct PfArgs {
   float* part_ml;        // [h_kv][n_split][R][2]: m (base 2, scaled), l
   int G, n_q, n_kv, R, off, causal, n_split, n_rt;
   float qscale;          // sm_scale * log2(e)
+  int window, sinks;     // kWin: query position p sees keys (p - window, p] and [0, sinks)
 };
+
+// The key tiles a row tile of positions [p_lo, p_hi] walks under a window: the
+// sinks' tiles, then the band's from the lowest row's first key on.  List
+// entry t is tile t below n_sink, t + skip from there.
+struct TileList {
+  int n, n_sink, skip;
+};
+__host__ __device__ __forceinline__ TileList tile_list(int p_lo, int kend, int window, int sinks) {
+  const int nt = (kend + kPfKeys - 1) / kPfKeys;
+  TileList l;
+  l.n_sink = min((sinks + kPfKeys - 1) / kPfKeys, nt);
+  l.skip = max(max(p_lo - window + 1, 0) / kPfKeys - l.n_sink, 0);
+  l.n = nt - l.skip;
+  return l;
+}
+
+// nonzero if one of the two 16-bit values of x is infinite or NaN: its
+// exponent, all ones, carries into its sign bit
+template <int DT>
+__device__ __forceinline__ uint32_t pf_nonfinite(uint32_t x) {
+  constexpr uint32_t e = DT == BMX_PREFILL_F16 ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = DT == BMX_PREFILL_F16 ? 0x04000400u : 0x00800080u;
+  return ((x & e) + one) & 0x80008000u;
+}
 
 template <int DT>
 __device__ __forceinline__ uint32_t pf_pack(float x, float y) {
@@ -98,9 +133,16 @@ __device__ __forceinline__ int ks_off(int key, int c) {
 }
 
 template <int DT>
+__device__ __forceinline__ float pf_elem(uint16_t b) {
+  if constexpr (DT == BMX_PREFILL_F16) return half_bits_to_float(b);
+  return __uint_as_float((uint32_t)b << 16);
+}
+
+template <int DT, bool kWin>
 __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void prefill_kernel(const PfArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ int s_bad[2];   // kWin: 1 + list entry of the stage's tile if its values hold an infinity or NaN
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
   const int total = gridDim.x, lin = blockIdx.x;
   const int logical = (total & 7) == 0 ? (lin & 7) * (total >> 3) + (lin >> 3) : lin;
@@ -112,7 +154,15 @@ void prefill_kernel(const PfArgs a) {
   // keys the tile's rows see: [0, kend); every row sees [0, edge)
   const int kend = a.causal ? min(a.n_kv, i_hi + a.off + 1) : a.n_kv;
   const int edge = a.causal ? min(a.n_kv, i_lo + a.off + 1) : a.n_kv;
-  const int nt = (kend + kPfKeys - 1) / kPfKeys;
+  TileList list{};
+  if constexpr (kWin) list = tile_list(i_lo + a.off, kend, a.window, a.sinks);
+  const int nt = kWin ? list.n : (kend + kPfKeys - 1) / kPfKeys;   // tiles walked
+  auto tile_at = [&](int t) { return kWin && t >= list.n_sink ? t + list.skip : t; };
+  // a tile of the list that some row does not see whole
+  auto partly = [&](int t) {
+    const int k0 = tile_at(t) * kPfKeys, k1 = k0 + kPfKeys;
+    return k1 > edge || (k1 > a.sinks && k0 < i_hi + a.off - a.window + 1);
+  };
   const int t0 = (int)((int64_t)split * nt / a.n_split), t1 = (int)((int64_t)(split + 1) * nt / a.n_split);
   const int t_mask = edge / kPfKeys;   // tiles from here on cross the edge or the end of the keys
 
@@ -121,11 +171,12 @@ void prefill_kernel(const PfArgs a) {
   // the lane's row sees
   const int r32 = lane & 31, hf = lane >> 5;
   u32x4_t qb[8];
-  int last_key;
+  int last_key, first_key = 0;   // kWin: keys below first_key are hidden, the sinks apart
   {
     const int r = min(R0 + 32 * wave + r32, a.R - 1);
     const int i = r / a.G, g = r - i * a.G;
     last_key = a.causal ? i + a.off : a.n_kv - 1;   // < n_kv either way
+    if constexpr (kWin) first_key = last_key - a.window + 1;
     const uint16_t* qp = a.q + (int64_t)(h * a.G + g) * a.qsh + (int64_t)i * a.qst + 8 * hf;
 #pragma unroll
     for (int dc = 0; dc < 8; ++dc) qb[dc] = *reinterpret_cast<const u32x4_t*>(qp + 16 * dc);
@@ -151,7 +202,7 @@ void prefill_kernel(const PfArgs a) {
   const int vr4 = tid & 15, vc = tid >> 4;
   u32x4_t kr[4], vr[4];
   auto issue = [&](int t) {
-    const int k0 = t * kPfKeys;
+    const int k0 = tile_at(t) * kPfKeys;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       kr[j] = __builtin_amdgcn_raw_buffer_load_b128(
@@ -161,9 +212,19 @@ void prefill_kernel(const PfArgs a) {
       vr[j] = __builtin_amdgcn_raw_buffer_load_b128(
           vrs, (uint32_t)(((int64_t)(k0 + 4 * vr4 + j) * a.st + 8 * vc) * 2), 0, 0);
   };
-  auto stash = [&](int stage) {
+  auto stash = [&](int stage, int t) {
     uint8_t* ks = smem + stage * kPfStage;
     uint8_t* vt = ks + kPfKsBytes;
+    if constexpr (kWin) {
+      if (partly(t)) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) bad |= pf_nonfinite<DT>(vr[j][p]);
+        if (bad != 0) s_bad[stage] = t + 1;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4_t*>(ks + ks_off(lr + 16 * j, lc)) = kr[j];
 #pragma unroll
@@ -221,8 +282,11 @@ void prefill_kernel(const PfArgs a) {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = t * kPfKeys + 32 * kb + 16 * (e >> 3) + 8 * hf + (e & 7);
+          const int key = tile_at(t) * kPfKeys + 32 * kb + 16 * (e >> 3) + 8 * hf + (e & 7);
           if (key > last_key) s[kb][e] = -INFINITY;
+          if constexpr (kWin) {
+            if (key < first_key && key >= a.sinks) s[kb][e] = -INFINITY;
+          }
         }
     }
     float mx = s[0][0];
@@ -266,8 +330,32 @@ void prefill_kernel(const PfArgs a) {
     l += ps;
     // the next tile goes to the other stage ahead of the values' MFMAs, so
     // that its writes overlap them
-    if (t + 1 < t1) stash(stage ^ 1);
+    if (t + 1 < t1) stash(stage ^ 1, t + 1);
     // ---- values: O^T += V^T . P^T over the tile's four 16-key sub-blocks
+    if constexpr (kWin && kMasked) {
+      if (s_bad[stage] == t + 1) {
+        // an infinite or NaN value in a tile with hidden keys: key by key, only those the row sees
+#pragma unroll 1
+        for (int kk = 0; kk < kPfKeys; ++kk) {
+          const int sb = kk >> 4, owner = (kk >> 3) & 1, key = tile_at(t) * kPfKeys + kk;
+          const u32x4_t w = sb == 0 ? pb[0] : sb == 1 ? pb[1] : sb == 2 ? pb[2] : pb[3];
+          const int d = (kk & 7) >> 1;
+          const uint32_t two = d == 0 ? w[0] : d == 1 ? w[1] : d == 2 ? w[2] : w[3];
+          const float p = __shfl(pf_elem<DT>((uint16_t)(kk & 1 ? two >> 16 : two)), r32 + 32 * owner);
+          const bool sees = key <= last_key && (key >= first_key || key < a.sinks);
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int c = 32 * cb + 8 * (e >> 2) + 4 * hf + (e & 3);
+              const float x = pf_elem<DT>(*reinterpret_cast<const uint16_t*>(vt + c * kPfVtPitch + 2 * kk));
+              if (sees) o[cb][e] = __builtin_fmaf(p, x, o[cb][e]);
+            }
+        }
+        __syncthreads();
+        return;
+      }
+    }
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int sb = 0; sb < 4; ++sb) {
@@ -282,14 +370,25 @@ void prefill_kernel(const PfArgs a) {
     __syncthreads();
   };
 
-  if (t0 < t1) {
-    issue(t0);
-    stash(0);
+  if constexpr (kWin) {
+    if (tid < 2) s_bad[tid] = 0;
     __syncthreads();
   }
-  const int t_split = max(t0, min(t1, t_mask));
-  for (int t = t0; t < t_split; ++t) tile(t, std::false_type{});
-  for (int t = t_split; t < t1; ++t) tile(t, std::true_type{});
+  if (t0 < t1) {
+    issue(t0);
+    stash(0, t0);
+    __syncthreads();
+  }
+  if constexpr (kWin) {
+    for (int t = t0; t < t1; ++t) {
+      if (partly(t)) tile(t, std::true_type{});
+      else tile(t, std::false_type{});
+    }
+  } else {
+    const int t_split = max(t0, min(t1, t_mask));
+    for (int t = t0; t < t_split; ++t) tile(t, std::false_type{});
+    for (int t = t_split; t < t1; ++t) tile(t, std::true_type{});
+  }
 
   // ---- rows out: lane (r32, hf) holds row r32, channels 32 cb + 8 j + 4 hf .. +3
   {
@@ -380,7 +479,17 @@ std::string pf_check(const bmx_prefill_args* a) {
   // one head's rows are addressed with 32-bit byte offsets (buffer loads)
   if ((int64_t)(a->n_kv + kPfKeys) * a->kv_stride_t * 2 > INT32_MAX) return "a head's K/V rows exceed 2 GiB";
   if ((int64_t)a->n_q * a->n_q_groups > INT32_MAX / 2) return "too many rows";
+  if (a->window < 0 || a->sinks < 0) return "window and sinks must be >= 0";
+  if (a->sinks > 0 && a->window == 0) return "sinks need a window";
+  if (a->window > 0 && !a->causal) return "a window needs causal";
   return "";
+}
+
+// a window that hides some key from some row (one as long as the keys hides none)
+bool pf_windowed(const bmx_prefill_args* a) { return a->window > 0 && a->window < a->n_kv; }
+// the window form of few rows (prefill_rows.hip)
+bool pf_few_rows(const bmx_prefill_args* a) {
+  return a->window > 0 && (int64_t)a->n_q * a->n_q_groups <= kRowsMax;
 }
 
 int pf_row_tiles(const bmx_prefill_args* a) {
@@ -392,7 +501,11 @@ int pf_splits(const bmx_prefill_args* a) {
   if (a->n_split > 0) return a->n_split;
   const int64_t base = (int64_t)pf_row_tiles(a) * a->h_kv;
   int s = (int)std::min<int64_t>((512 + base - 1) / base, kPfMaxSplit);
-  const int nt = (a->n_kv + kPfKeys - 1) / kPfKeys;
+  int nt = (a->n_kv + kPfKeys - 1) / kPfKeys;
+  if (pf_windowed(a)) {   // the longest list: the last row tile's
+    const int p_lo = a->n_kv - std::min(a->n_q, (kPfRows + a->n_q_groups - 1) / a->n_q_groups + 1);
+    nt = tile_list(p_lo, a->n_kv, a->window, std::min(a->sinks, a->n_kv)).n;
+  }
   s = std::min(s, std::max(1, nt / 4));
   return std::max(s, 1);
 }
@@ -404,6 +517,7 @@ using namespace bmx;
 
 extern "C" size_t bmx_prefill_workspace_bytes(const bmx_prefill_args* a) {
   if (!pf_check(a).empty()) return 0;
+  if (pf_few_rows(a)) return rows_workspace_bytes(a);
   const int s = pf_splits(a);
   if (s == 1) return 0;
   return (size_t)a->h_kv * s * ((size_t)a->n_q * a->n_q_groups) * (kPfD + 2) * sizeof(float);
@@ -412,10 +526,15 @@ extern "C" size_t bmx_prefill_workspace_bytes(const bmx_prefill_args* a) {
 extern "C" int bmx_prefill(const bmx_prefill_args* a, void* stream) {
   const std::string why = pf_check(a);
   if (!why.empty()) return pf_fail(BMX_PREFILL_E_INVALID, why);
-  const int S = pf_splits(a);
+  const bool few = pf_few_rows(a), windowed = pf_windowed(a);
+  const int S = few ? 0 : pf_splits(a);
   const size_t need = bmx_prefill_workspace_bytes(a);
   if (need && (!a->workspace || a->workspace_bytes < need))
     return pf_fail(BMX_PREFILL_E_INVALID, "workspace too small (bmx_prefill_workspace_bytes)");
+  if (few) {
+    if (rows_launch(a, (hipStream_t)stream) != hipSuccess) return pf_fail(BMX_PREFILL_E_HIP, "kernel launch failed");
+    return 0;
+  }
   PfArgs k{};
   k.q = static_cast<const uint16_t*>(a->q);
   k.qsh = a->q_stride_h;
@@ -434,6 +553,8 @@ extern "C" int bmx_prefill(const bmx_prefill_args* a, void* stream) {
   k.n_split = S;
   k.n_rt = pf_row_tiles(a);
   k.qscale = a->sm_scale * 1.4426950408889634f;
+  k.window = a->window;
+  k.sinks = std::min(a->sinks, a->n_kv);
   if (S > 1) {
     k.part_o = static_cast<float*>(a->workspace);
     k.part_ml = k.part_o + (size_t)a->h_kv * S * k.R * kPfD;
@@ -441,14 +562,16 @@ extern "C" int bmx_prefill(const bmx_prefill_args* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   const int64_t blocks = (int64_t)k.n_rt * S * a->h_kv;
   if (blocks > INT32_MAX) return pf_fail(BMX_PREFILL_E_INVALID, "too many workgroups");
-  const void* fn = a->dtype == BMX_PREFILL_F16 ? (const void*)prefill_kernel<BMX_PREFILL_F16>
-                                                : (const void*)prefill_kernel<BMX_PREFILL_BF16>;
-  if (bmx_ensure_dynamic_lds(fn, kPfLds) != hipSuccess)
+  auto launch = [&](auto kernel) {
+    if (bmx_ensure_dynamic_lds((const void*)kernel, kPfLds) != hipSuccess) return false;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kPfThreads), kPfLds, st, k);
+    return true;
+  };
+  const bool f16 = a->dtype == BMX_PREFILL_F16;
+  if (!(windowed ? (f16 ? launch(prefill_kernel<BMX_PREFILL_F16, true>) : launch(prefill_kernel<BMX_PREFILL_BF16, true>))
+                 : (f16 ? launch(prefill_kernel<BMX_PREFILL_F16, false>)
+                        : launch(prefill_kernel<BMX_PREFILL_BF16, false>))))
     return pf_fail(BMX_PREFILL_E_HIP, "cannot reserve the kernel's LDS");
-  if (a->dtype == BMX_PREFILL_F16)
-    hipLaunchKernelGGL(prefill_kernel<BMX_PREFILL_F16>, dim3((unsigned)blocks), dim3(kPfThreads), kPfLds, st, k);
-  else
-    hipLaunchKernelGGL(prefill_kernel<BMX_PREFILL_BF16>, dim3((unsigned)blocks), dim3(kPfThreads), kPfLds, st, k);
   if (hipGetLastError() != hipSuccess) return pf_fail(BMX_PREFILL_E_HIP, "kernel launch failed");
   if (S > 1) {
     PfCombineArgs c{};

@@ -6,9 +6,10 @@ src/bmx/cache/chunked_attention.py:320-395) dequantizes the committed pages
 to dense rows and calls torch SDPA with the model's mask.  The packed cache
 keeps the dequant and attends here instead for the masks a cached prefill
 carries: the causal mask of the last ``n_q`` positions (bottom-right aligned;
-``n_q == n_kv`` is the ordinary causal mask) or none.  The kernel enqueues on
-torch's current stream; any non-zero status raises with the library's
-message (no fallback).
+``n_q == n_kv`` is the ordinary causal mask) or none; and, for layers that
+slide, the causal mask within a window, with or without a few first tokens
+that stay visible (sinks).  The kernel enqueues on torch's current stream;
+any non-zero status raises with the library's message (no fallback).
 """
 
 from __future__ import annotations
@@ -39,12 +40,17 @@ def supported(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, causal: bool,
-              n_split: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+              n_split: int = 0, out: torch.Tensor | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """softmax(q k^T * scale [+ bottom-right causal mask]) v over grouped heads.
 
     q (h_kv * G, n_q, 128); k and v (h_kv, n_kv, 128) with the same strides;
     fp16 or bf16, rows contiguous.  Query head ``h * G + g`` reads kv head
-    ``h``.  With ``causal`` query i sees keys ``j <= i + n_kv - n_q``.
+    ``h``.  With ``causal`` query i sees keys ``j <= p = i + n_kv - n_q``; with
+    ``window`` > 0 as well only those with ``j > p - window`` (HF's
+    sliding_window: the query's own key is one of the window) or ``j < sinks``.
+    Rows that no query sees may hold anything.  Few rows (n_q * G up to 8, a
+    token's attention) under a window run on a form of their own, the keys
+    spread over the chip.
     Returns (h_kv * G, n_q, 128) in q's dtype, contiguous."""
     _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape, "q (Hq, n_q, 128), k and v (h_kv, n_kv, 128)")
     _need(q.shape[-1] == HEAD_DIM and k.shape[-1] == HEAD_DIM, "head_dim must be 128")
@@ -54,6 +60,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     hq, n_q, _ = q.shape
     h_kv, n_kv, _ = k.shape
     _need(hq % h_kv == 0, "query heads must be a multiple of kv heads")
+    window, sinks = int(window), int(sinks)
+    _need(window >= 0 and sinks >= 0, "window and sinks must be >= 0")
+    _need(sinks == 0 or window > 0, "sinks need a window")
+    _need(window == 0 or causal, "a window needs causal")
+    # past the keys both are without effect (and the C ABI's are 32-bit)
+    window, sinks = min(window, 2**31 - 1), min(sinks, 2**31 - 1)
     if out is None:
         out = torch.empty(hq, n_q, HEAD_DIM, dtype=q.dtype, device=q.device)
     _need(out.shape == (hq, n_q, HEAD_DIM) and out.dtype == q.dtype and out.is_contiguous(), "out (Hq, n_q, 128)")
@@ -64,7 +76,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     a.h_kv, a.n_q_groups, a.n_q, a.n_kv = h_kv, hq // h_kv, n_q, n_kv
     a.head_dim, a.dtype, a.causal, a.sm_scale = HEAD_DIM, DTYPES[q.dtype], int(bool(causal)), float(scale)
     a.n_split = int(n_split)
+    a.window, a.sinks = window, sinks
     L = _lib.lib()
+    if window:   # scratch of its own, from torch's allocator: calls on two streams or in two graphs share none
+        with torch.cuda.device(q.device):
+            need = int(L.bmx_prefill_workspace_bytes(ct.byref(a)))
+            if need:
+                ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+                a.workspace, a.workspace_bytes = ws.data_ptr(), need
+            _lib.check(L.bmx_prefill(ct.byref(a), _stream(q.device)), "bmx_prefill")
+        return out
     need = int(L.bmx_prefill_workspace_bytes(ct.byref(a)))
     if need:
         ws = _WS.setdefault(q.device, DecodeWorkspace()).get(need, q.device)

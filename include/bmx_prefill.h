@@ -9,6 +9,8 @@
 // a cached prefill carries: the causal mask of the last n_q positions over
 // n_kv keys (bottom-right aligned; n_q == n_kv is the plain causal mask), or
 // no mask.  Grouped-query heads read their K/V head in place (no expansion).
+// Models whose layers slide add a window, with or without a few first tokens
+// that stay visible (sinks).
 #ifndef BMX_PREFILL_H
 #define BMX_PREFILL_H
 
@@ -44,6 +46,10 @@ typedef struct bmx_prefill_args {
   int n_split;            // key ranges per row tile (1..16), 0: chosen by the library
   void* workspace;        // bmx_prefill_workspace_bytes(); may be NULL when that is 0
   size_t workspace_bytes;
+  int window;             // > 0 (needs causal): query i, at position p = i + n_kv - n_q, sees keys
+                          // p - window < j <= p and the sinks; 0: no window.  K and V rows that no
+                          // query sees may hold anything, infinities and NaN among it
+  int sinks;              // first keys that every query at or past them sees (needs a window); 0: none
 } bmx_prefill_args;
 
 // Device scratch the call needs (split partials), for the n_split it will
