@@ -67,6 +67,40 @@ class DecodeArgs(ct.Structure):
     ]
 
 
+class DecodeSharedArgs(ct.Structure):
+    _fields_ = [
+        ("geom", Geom),
+        ("batch", ct.c_int32),
+        ("io_dtype", ct.c_int32),
+        ("q", ct.c_void_p),
+        ("out", ct.c_void_p),
+        ("pages", ct.c_void_p),
+        ("n_pool_pages", ct.c_int32),
+        ("max_pages", ct.c_int32),
+        ("page_table", ct.c_void_p),
+        ("packed_len", ct.c_void_p),
+        ("max_packed_len", ct.c_int32),
+        ("shared_len", ct.c_int32),
+        ("basis", ct.c_void_p),
+        ("rope", ct.c_void_p),
+        ("rope_pages", ct.c_int32),
+        ("rope_scaling", ct.c_float),
+        ("sm_scale", ct.c_float),
+        ("codebook", ct.c_float * 4),
+        ("v_sign_bits", ct.c_uint32 * 4),
+        ("k_tail", ct.c_void_p),
+        ("v_tail", ct.c_void_p),
+        ("tail_stride_b", ct.c_int64),
+        ("tail_stride_h", ct.c_int64),
+        ("tail_stride_t", ct.c_int64),
+        ("tail_len", ct.c_void_p),
+        ("tail_len_value", ct.c_int32),
+        ("tail_cap", ct.c_int32),
+        ("workspace", ct.c_void_p),
+        ("workspace_bytes", ct.c_size_t),
+    ]
+
+
 class AppendArgs(ct.Structure):
     _fields_ = [
         ("geom", Geom),
@@ -286,6 +320,9 @@ EXPORTS = {
     "bmx_k2b_decode_workspace_bytes": (ct.c_size_t, [ct.POINTER(DecodeArgs)]),
     "bmx_k2b_decode": (ct.c_int, [ct.POINTER(DecodeArgs), ct.c_void_p]),
     "bmx_k2b_decode_noalloc": (ct.c_int, [ct.POINTER(DecodeArgs), ct.c_void_p]),
+    "bmx_k2b_rope_table": (ct.c_int, [ct.POINTER(ct.c_float), ct.c_int32, ct.c_void_p, ct.c_void_p]),
+    "bmx_k2b_decode_shared_workspace_bytes": (ct.c_size_t, [ct.POINTER(DecodeSharedArgs)]),
+    "bmx_k2b_decode_shared": (ct.c_int, [ct.POINTER(DecodeSharedArgs), ct.c_void_p]),
     "bmx_k2b_append": (ct.c_int, [ct.POINTER(AppendArgs), ct.c_void_p]),
     "bmx_k2b_dequant": (ct.c_int, [ct.POINTER(DequantArgs), ct.c_void_p]),
     "bmx_rtn_page_bytes": (ct.c_size_t, [ct.POINTER(RtnGeom)]),

@@ -32,6 +32,7 @@ COMMON = [
 SOURCES = {
     "k2b_api.hip": [],
     "k2b_decode.hip": ["-ffp-contract=fast"],
+    "k2b_shared.hip": ["-ffp-contract=fast"],
     "k2b_append.hip": ["-ffp-contract=off"],
     "k2b_dequant.hip": ["-ffp-contract=off"],
     "rtn.hip": ["-ffp-contract=off"],

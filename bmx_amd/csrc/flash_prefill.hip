@@ -32,10 +32,10 @@
 // the tiles that some row of it sees, the sinks' tiles and then the band's
 // (TileList), and masks those that cross an edge of the band, of the sinks or
 // of the keys.  A hidden key weighs 0, but 0 times an infinite or NaN value is
-// NaN: a masked tile's values are looked over as they are staged, and a tile
-// that holds one goes through a loop that takes only the keys a row sees
-// (values hidden from every row, such as evicted rows of a cache, may hold
-// anything).
+// NaN: a masked tile's values are looked over as they are staged, those that
+// are not finite staged as 0, and a tile that held one adds them afterwards to
+// the rows that see them (values hidden from every row, such as evicted rows
+// of a cache, may hold anything).
 
 #include "bmx_prefill.h"
 #include "k2b_common.h"
@@ -222,7 +222,13 @@ void prefill_kernel(const PfArgs a) {
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int p = 0; p < 4; ++p) bad |= pf_nonfinite<DT>(vr[j][p]);
-        if (bad != 0) s_bad[stage] = t + 1;
+        if (bad != 0) {
+          s_bad[stage] = t + 1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) vr[j][p] &= ~((pf_nonfinite<DT>(vr[j][p]) >> 15) * 0xffffu);
+        }
       }
     }
 #pragma unroll
@@ -277,7 +283,7 @@ void prefill_kernel(const PfArgs a) {
     }
     __builtin_amdgcn_s_setprio(0);
     // ---- online softmax (base 2) of the lane's row; P^T as the values' B operand
-    if constexpr (kMasked) {
+    if (kMasked || (kWin && partly(t))) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -332,30 +338,6 @@ void prefill_kernel(const PfArgs a) {
     // that its writes overlap them
     if (t + 1 < t1) stash(stage ^ 1, t + 1);
     // ---- values: O^T += V^T . P^T over the tile's four 16-key sub-blocks
-    if constexpr (kWin && kMasked) {
-      if (s_bad[stage] == t + 1) {
-        // an infinite or NaN value in a tile with hidden keys: key by key, only those the row sees
-#pragma unroll 1
-        for (int kk = 0; kk < kPfKeys; ++kk) {
-          const int sb = kk >> 4, owner = (kk >> 3) & 1, key = tile_at(t) * kPfKeys + kk;
-          const u32x4_t w = sb == 0 ? pb[0] : sb == 1 ? pb[1] : sb == 2 ? pb[2] : pb[3];
-          const int d = (kk & 7) >> 1;
-          const uint32_t two = d == 0 ? w[0] : d == 1 ? w[1] : d == 2 ? w[2] : w[3];
-          const float p = __shfl(pf_elem<DT>((uint16_t)(kk & 1 ? two >> 16 : two)), r32 + 32 * owner);
-          const bool sees = key <= last_key && (key >= first_key || key < a.sinks);
-#pragma unroll
-          for (int cb = 0; cb < 4; ++cb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int c = 32 * cb + 8 * (e >> 2) + 4 * hf + (e & 3);
-              const float x = pf_elem<DT>(*reinterpret_cast<const uint16_t*>(vt + c * kPfVtPitch + 2 * kk));
-              if (sees) o[cb][e] = __builtin_fmaf(p, x, o[cb][e]);
-            }
-        }
-        __syncthreads();
-        return;
-      }
-    }
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int sb = 0; sb < 4; ++sb) {
@@ -367,6 +349,28 @@ void prefill_kernel(const PfArgs a) {
       for (int cb = 0; cb < 4; ++cb) o[cb] = pf_mma32<DT>(va[cb], pb[sb], o[cb]);
     }
     __builtin_amdgcn_s_setprio(0);
+    if constexpr (kWin) {
+      if (s_bad[stage] == t + 1) {   // rare: whatever weight a row gives such a value, its sum is that value's
+#pragma unroll 1
+        for (int kk = 0; kk < kPfKeys; ++kk) {
+          const int key = tile_at(t) * kPfKeys + kk;
+          if (key > last_key || (key < first_key && key >= a.sinks)) continue;
+          const uint16_t* vp = a.v + (int64_t)h * a.sh + (int64_t)key * a.st + 4 * hf;
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vp + 32 * cb + 8 * j);
+              if ((pf_nonfinite<DT>(w[0]) | pf_nonfinite<DT>(w[1])) == 0) continue;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = pf_elem<DT>((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+                if (!(__builtin_fabsf(x) < INFINITY)) o[cb][4 * j + e] += x;
+              }
+            }
+        }
+      }
+    }
     __syncthreads();
   };
 
@@ -380,10 +384,7 @@ void prefill_kernel(const PfArgs a) {
     __syncthreads();
   }
   if constexpr (kWin) {
-    for (int t = t0; t < t1; ++t) {
-      if (partly(t)) tile(t, std::true_type{});
-      else tile(t, std::false_type{});
-    }
+    for (int t = t0; t < t1; ++t) tile(t, std::false_type{});
   } else {
     const int t_split = max(t0, min(t1, t_mask));
     for (int t = t0; t < t_split; ++t) tile(t, std::false_type{});

@@ -294,6 +294,13 @@ struct AppendKArgs {
 
 // The code thresholds of a codebook at head_dim d (k2b_append.hip).
 void set_code_cuts(AppendKArgs& k, const float codebook[4], int d);
+// The fp16 value levels of a codebook as an affine image (level_map, k2b_decode.hip).
+struct LevelMap {
+  uint32_t hi[4];
+  float kappa, mu;
+  double err;   // max |hi_c - (kappa level_c + mu)| / max |kappa level|
+};
+LevelMap level_map(const float cb[4]);
 // Norms and codes of n_pages16 16-token pages of h_kv heads (head_dim 128) into
 // the VNORM and VCODE sections of a.L (k2b_append.hip).
 hipError_t launch_k2b_values(const AppendKArgs& a, int n_pages16, int h_kv, hipStream_t st);

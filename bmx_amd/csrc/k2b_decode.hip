@@ -721,12 +721,6 @@ extern "C" size_t bmx_k2b_decode_workspace_bytes(const bmx_k2b_decode_args* a) {
 // found by a search over fp16 values for the two extreme levels (the two middle
 // levels follow) and cached per codebook.
 // ---------------------------------------------------------------------------
-struct LevelMap {
-  uint32_t hi[4];
-  float kappa, mu;
-  double err;   // max |hi_c - (kappa level_c + mu)| / max |kappa level|
-};
-
 static double round_half(double v) {   // nearest fp16 value (normal range), ties to even
   return (double)(_Float16)v;
 }
@@ -806,7 +800,7 @@ static LevelMap search_level_map(const float cb[4]) {
   return best;
 }
 
-static LevelMap level_map(const float cb[4]) {
+LevelMap bmx::level_map(const float cb[4]) {
   struct Entry {
     float cb[4];
     LevelMap m;

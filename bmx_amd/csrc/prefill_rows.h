@@ -7,9 +7,9 @@
 
 namespace bmx {
 
-// query rows (positions times heads of a KV head) the form takes: a lane keeps
-// 8 channels of every row's query and sum
-constexpr int kRowsMax = 8;
+// query rows (positions times heads of a KV head) the form takes: the columns
+// of one 16x16 matrix product
+constexpr int kRowsMax = 16;
 
 size_t rows_workspace_bytes(const bmx_prefill_args* a);
 hipError_t rows_launch(const bmx_prefill_args* a, hipStream_t st);

@@ -328,6 +328,120 @@ class DecodePlan:
         return res
 
 
+@dataclass(frozen=True)
+class RopeTable:
+    """Rotations of positions 0 .. n_tokens - 1 for decode_shared (rope_table): one a
+    model and device, read by every layer's calls."""
+
+    data: torch.Tensor      # uint8 (n_tokens / 16, 4096), the layout of bmx_k2b_rope_table
+    inv_freq: tuple
+
+    @property
+    def n_tokens(self) -> int:
+        return self.data.shape[0] * PAGE_TOKENS
+
+
+ROPE_PAGE_BYTES = 4096   # BMX_K2B_ROPE_PAGE_BYTES
+
+
+def rope_table(consts: CodecConsts, n_tokens: int, device) -> RopeTable:
+    """The rotation table of consts' frequencies for positions below n_tokens
+    (rounded up to whole pages): 256 bytes a position."""
+    device = torch.device(device)
+    _need(consts.head_dim == HEAD_DIM, "the rotation table is made for head_dim 128")
+    _need(device.type == "cuda", "device must be a HIP device")
+    n = max(1, -(-int(n_tokens) // PAGE_TOKENS))
+    _need(n <= 1 << 20, "n_tokens must be at most 2^24")
+    data = torch.empty(n, ROPE_PAGE_BYTES, dtype=torch.uint8, device=device)
+    freq = (ct.c_float * 64)(*consts.inv_freq)
+    with torch.cuda.device(data.device):
+        _lib.check(_lib.lib().bmx_k2b_rope_table(freq, n, data.data_ptr(), _stream(data.device)), "bmx_k2b_rope_table")
+    return RopeTable(data, tuple(consts.inv_freq))
+
+
+def decode_shared(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, packed_len: torch.Tensor,
+                  max_packed_len: int, shared_len: int, basis16: torch.Tensor, consts: CodecConsts, sm_scale: float,
+                  *, rank: int, rope: RopeTable, k_tail: torch.Tensor | None = None,
+                  v_tail: torch.Tensor | None = None, tail_len=None, tail_cap: int = 0,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """One decode step of a batch whose sequences share their first shared_len
+    tokens: decode() over the same tables, the shared pages read and rebuilt
+    once for the batch.
+
+    q (B, h_kv, G, 128) post-RoPE in fp16 or bf16 -> the same shape and dtype;
+    page_table (B, max_pages) int32, whose rows begin with the same shared_len
+    / 16 pages (row 0's are read); packed_len (B,) int32 committed tokens,
+    shared ones included (whole 64-token groups are attended; a sequence may
+    hold less than shared_len, or nothing); basis16 (C, rank) fp16, every
+    sequence's (it is frozen at the first page, which they share); rope: the
+    rotations of at least max_packed_len positions; k_tail / v_tail (B, h_kv,
+    >= tail_cap, 128) in q's dtype with tail_len rows (a device int32 (B,)
+    tensor or a host int).  The recipe's page (128, 16 or 32, 64, 3).  A
+    sequence that holds nothing gives zeros."""
+    _need(q.dim() == 4 and q.shape[3] == HEAD_DIM and q.dtype in (torch.float16, torch.bfloat16) and q.is_contiguous(),
+          "q must be contiguous fp16 or bf16 (B, h_kv, G, 128)")
+    B, h_kv, G, d = q.shape
+    dev = q.device
+    _need(q.is_cuda, "operands must be on a HIP device")
+    _need(B > 0, "the batch is empty")
+    _need(consts.head_dim == d, "consts were made for another head_dim")
+    _need(pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous()
+          and pages.shape[1] == page_bytes(h_kv, rank), "pages must be a contiguous (n_pages, page_bytes) uint8 pool")
+    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
+          and page_table.is_contiguous(), "page_table must be contiguous int32 (B, max_pages)")
+    _need(packed_len.dtype == torch.int32 and packed_len.numel() == B and packed_len.is_contiguous(),
+          "packed_len must be int32[B]")
+    _need(basis16.shape == (h_kv * d, rank) and basis16.dtype == torch.float16 and basis16.is_contiguous(),
+          "basis16 must be contiguous fp16 (C, rank)")
+    _need(rope.inv_freq == tuple(consts.inv_freq), "rope was made for other frequencies")
+    _need(rope.n_tokens >= max_packed_len, "rope holds fewer positions than max_packed_len")
+    tensors = [pages, page_table, packed_len, basis16, rope.data]
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous(),
+          "out must be contiguous and of q's shape and dtype")
+    a = _lib.DecodeSharedArgs()
+    a.geom = geom(h_kv, rank, G)
+    a.batch, a.io_dtype = B, _IO_DTYPES[q.dtype]
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.pages, a.n_pool_pages = pages.data_ptr(), pages.shape[0]
+    a.page_table, a.max_pages = page_table.data_ptr(), page_table.shape[1]
+    a.packed_len, a.max_packed_len, a.shared_len = packed_len.data_ptr(), int(max_packed_len), int(shared_len)
+    a.basis, a.rope, a.rope_pages = basis16.data_ptr(), rope.data.data_ptr(), rope.data.shape[0]
+    a.rope_scaling, a.sm_scale = consts.rope_scaling, float(sm_scale)
+    a.codebook[:] = consts.codebook
+    a.v_sign_bits[:] = consts.sign_bits
+    if tail_cap > 0:
+        _need(k_tail is not None and v_tail is not None and k_tail.dim() == 4 and k_tail.shape == v_tail.shape
+              and k_tail.stride() == v_tail.stride(), "k_tail/v_tail must share shape and strides")
+        _need(k_tail.dtype == q.dtype and v_tail.dtype == q.dtype and k_tail.shape[:2] == (B, h_kv)
+              and k_tail.shape[2] >= tail_cap and k_tail.shape[3] == d and k_tail.stride(3) == 1,
+              "k_tail/v_tail must be (B, h_kv, >=tail_cap, 128) in q's dtype with contiguous last dim")
+        a.k_tail, a.v_tail = k_tail.data_ptr(), v_tail.data_ptr()
+        # strides of size-1 dimensions are never used: taken as 0
+        a.tail_stride_b, a.tail_stride_h, a.tail_stride_t = (
+            0 if n == 1 else st for n, st in zip(k_tail.shape[:3], k_tail.stride()[:3]))
+        tensors += [k_tail, v_tail]
+    a.tail_cap = int(tail_cap)
+    if isinstance(tail_len, torch.Tensor):
+        _need(tail_len.dtype == torch.int32 and tail_len.numel() == B and tail_len.is_contiguous(),
+              "tail_len must be a device int32[B] tensor or a host int")
+        a.tail_len = tail_len.data_ptr()
+        tensors.append(tail_len)
+    else:
+        a.tail_len_value = 0 if tail_len is None else int(tail_len)
+        _need(0 <= a.tail_len_value <= tail_cap, "tail_len must be within 0..tail_cap")
+    _need(all(t.device == dev for t in tensors) and out.device == dev, "operands must be on one device")
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        # scratch of the call's own, from torch's allocator: calls on two streams or in two graphs share none
+        need = int(lib.bmx_k2b_decode_shared_workspace_bytes(ct.byref(a)))
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _lib.check(lib.bmx_k2b_decode_shared(ct.byref(a), _stream(dev)), "bmx_k2b_decode_shared")
+    return out
+
+
 ROPE_NONE, ROPE_EXACT, ROPE_FP16_TABLES = 0, 1, 2
 
 

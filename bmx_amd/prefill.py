@@ -48,7 +48,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     ``h``.  With ``causal`` query i sees keys ``j <= p = i + n_kv - n_q``; with
     ``window`` > 0 as well only those with ``j > p - window`` (HF's
     sliding_window: the query's own key is one of the window) or ``j < sinks``.
-    Rows that no query sees may hold anything.  Few rows (n_q * G up to 8, a
+    Rows that no query sees may hold anything.  Few rows (n_q * G up to 16, a
     token's attention) under a window run on a form of their own, the keys
     spread over the chip.
     Returns (h_kv * G, n_q, 128) in q's dtype, contiguous."""

@@ -217,6 +217,62 @@ int bmx_k2b_decode(const bmx_k2b_decode_args* args, void* stream);
 int bmx_k2b_decode_noalloc(const bmx_k2b_decode_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Shared-prefix decode: one query step of a batch of sequences whose first
+ * shared_len tokens are the same (a system prompt, a document, the prompt of
+ * several samples).  The result is that of bmx_k2b_decode over the same
+ * tables; the pages of the first shared_len tokens are read and rebuilt once
+ * for the whole batch, through row 0 of page_table (the other rows' first
+ * shared_len / 16 entries are not read).  The recipe's page only.  For each
+ * sequence b: the first packed_len[b] committed tokens (those past shared_len
+ * on row b's own pages) and tail_len[b] window rows, one softmax over their
+ * union; a sequence that holds nothing gives zeros.
+ * ---------------------------------------------------------------------- */
+
+/* Rotation table of positions 0 .. 16 n_pages - 1, read by the shared-prefix
+ * decode of every layer: fp16 (cos, sin) of HF's angle fl32(inv_freq_j * pos),
+ * without rope_scaling, 4096 bytes a page: [page][b][lane 16q+n][i] holds
+ * token n, pair j = 16b + 4q + i (b, i < 4).  Written once a model. */
+#define BMX_K2B_ROPE_PAGE_BYTES 4096
+int bmx_k2b_rope_table(const float inv_freq[64], int32_t n_pages, void* out, void* stream);
+
+typedef struct {
+  bmx_k2b_geom geom;          /* head_dim 128, group 64, 3 bits, rank 16 or 32, h_kv 1..16 */
+  int32_t batch;
+  int32_t io_dtype;           /* BMX_K2B_IO_F16 or _BF16: q, out, k_tail and v_tail */
+  const void* q;              /* device [batch][h_kv][G][128] post-RoPE, 16-byte aligned */
+  void* out;                  /* device [batch][h_kv][G][128] */
+  const uint8_t* pages;       /* device page pool, n_pool_pages pages (entries clamped into it) */
+  int32_t n_pool_pages;
+  int32_t max_pages;          /* row stride of page_table */
+  const int32_t* page_table;  /* device [batch][max_pages] */
+  const int32_t* packed_len;  /* device [batch] committed tokens, whole 64-token groups of which are
+                                 attended; clamped to 0..max_packed_len; may be below shared_len */
+  int32_t max_packed_len;     /* host upper bound of packed_len, a multiple of 128, >= shared_len */
+  int32_t shared_len;         /* tokens of the common prefix, a multiple of 128, 0 for none */
+  const uint16_t* basis;      /* device fp16 [C][R], the key basis of every sequence (a basis is
+                                 frozen at a sequence's first page, which they share) */
+  const void* rope;           /* device bmx_k2b_rope_table() of these inv_freq */
+  int32_t rope_pages;         /* its pages, >= max_packed_len / 16 */
+  float rope_scaling;
+  float sm_scale;
+  float codebook[4];
+  uint32_t v_sign_bits[4];
+  const void* k_tail;         /* device post-RoPE window rows in io_dtype, strides in elements */
+  const void* v_tail;         /* (multiples of 8, rows 16-byte aligned) */
+  int64_t tail_stride_b;
+  int64_t tail_stride_h;
+  int64_t tail_stride_t;
+  const int32_t* tail_len;    /* device [batch], clamped to 0..tail_cap, or NULL: tail_len_value each */
+  int32_t tail_len_value;
+  int32_t tail_cap;           /* 0..4096 */
+  void* workspace;            /* device scratch, bmx_k2b_decode_shared_workspace_bytes() */
+  size_t workspace_bytes;
+} bmx_k2b_decode_shared_args;
+
+size_t bmx_k2b_decode_shared_workspace_bytes(const bmx_k2b_decode_shared_args* args);
+int bmx_k2b_decode_shared(const bmx_k2b_decode_shared_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
  * Quantize-on-append (page commit).  Replaces the write path of
  * PackedStreamingLayer.update (cache/packed_streaming.py:582-730):
  * _pack_k_block -> quantize_packed("lowrank_rtn_channel") (codecs.py:786-796,

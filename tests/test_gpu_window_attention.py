@@ -5,9 +5,10 @@ alone, in both forms: row tiles on MFMA and few rows.
 The bound of every element, with u = eps / 2 of the type, P the exact weights
 and A = P |v|:
   * the output's rounding: u |out|;
-  * MFMA form: each weight is rounded to 16 bits before it meets v: u A, and
-    in fp16, where weights below 2^-14 of the row's largest are subnormal, up
-    to 2^-25 a key and unit of v (the sum of weights is at least 1);
+  * each weight is rounded to 16 bits before it meets v: u A, and in fp16 the
+    smallest ones are subnormal: with row tiles (weights below 2^-14 of the
+    row's largest) up to 2^-25 a key and unit of v, where the sum of weights
+    is at least 1; with few rows (below 2^-29) 2^15 times less;
   * a score is a sum of 128 products in fp32, off by at most 130 2^-24 of the
     sum of their sizes, d; a relative weight is off by 2 d and by the fp32
     exponential, sums and division (8 2^-23 allowed for): (2 d + 2^-20) A."""
@@ -42,7 +43,7 @@ def _check(out, q, k, v, window, sinks):
     reference (their values are zeroed per row where they are not finite)."""
     hq, n_q, _ = q.shape
     h_kv, n_kv, _ = k.shape
-    G, few = hq // h_kv, n_q * (hq // h_kv) <= 8
+    G, few = hq // h_kv, n_q * (hq // h_kv) <= 16
     u = torch.finfo(q.dtype).eps / 2
     seen = _seen(n_q, n_kv, window, sinks)
     worst = 0.0
@@ -56,12 +57,9 @@ def _check(out, q, k, v, window, sinks):
         w = torch.softmax(s, -1)
         ref, A = w @ vd, w @ vd.abs()
         bound = u * ref.abs() + (2 * d + 2.0 ** -20) * A + 1e-30
-        if not few:
-            bound = bound + u * A
-            if q.dtype == torch.float16:
-                bound = bound + 2.0 ** -25 * seen.sum(-1)[:, None] * vd.abs().max()
-        if q.dtype == torch.float16:   # outputs below 2^-14 are subnormal
-            bound = bound + 2.0 ** -25
+        bound = bound + u * A
+        if q.dtype == torch.float16:   # subnormal weights; outputs below 2^-14 are subnormal too
+            bound = bound + 2.0 ** (-40 if few else -25) * seen.sum(-1)[:, None] * vd.abs().max() + 2.0 ** -25
         err = (out[h].double() - ref).abs()
         assert torch.isfinite(out[h].double()).all(), f"head {h}: not finite"
         worst = max(worst, float((err / bound).max()))
@@ -80,7 +78,10 @@ CASES = [
     (2, 2, 200, 250, 100000, 5, 0),    # a window longer than the keys: none
     (2, 2, 200, 250, 249, 5, 0),
     (1, 8, 9, 40, 16, 300, 0),         # more sinks than keys
-    (1, 16, 1, 1000, 200, 4, 16),      # one position, more rows than the few-row form takes
+    (1, 17, 1, 1000, 200, 4, 16),      # one position, more rows than the few-row form takes
+    (1, 16, 1, 1000, 200, 4, 16),
+    (2, 4, 4, 6000, 700, 4, 0),
+    (1, 5, 3, 400, 90, 33, 3),
     # few rows
     (8, 4, 1, 5000, 1024, 4, 0),
     (2, 7, 1, 700, 256, 1, 0),
