@@ -1,6 +1,6 @@
 """ctypes binding of libbmx_k2b.so (the C-ABI declared in include/bmx_k2b.h,
-include/bmx_rtn.h, include/bmx_spectral.h, include/bmx_prefill.h and
-include/bmx_bench.h).
+include/bmx_rtn.h, include/bmx_spectral.h, include/bmx_prefill.h,
+include/bmx_pages.h and include/bmx_bench.h).
 
 The library is the product path: there is no fallback.  ``lib()`` raises if the
 shared object was not built (python -m bmx_amd.build) and every wrapper raises
@@ -312,6 +312,31 @@ class PrefillArgs(ct.Structure):
     ]
 
 
+class PagesState(ct.Structure):
+    _fields_ = [("table", ct.c_void_p), ("n_pages", ct.c_void_p), ("refs", ct.c_void_p), ("free", ct.c_void_p),
+                ("n_free", ct.c_void_p)]
+
+
+class PagesUpdateArgs(ct.Structure):
+    """bmx_pages_update_args (include/bmx_pages.h)."""
+    _fields_ = [
+        ("in", PagesState), ("out", PagesState),
+        ("rows", ct.c_int32), ("new_rows", ct.c_int32), ("cap", ct.c_int32), ("n_pool", ct.c_int32),
+        ("index", ct.c_void_p), ("grow", ct.c_void_p), ("status", ct.c_void_p),
+        ("workspace", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+    ]
+
+
+class PagesCompactArgs(ct.Structure):
+    """bmx_pages_compact_args (include/bmx_pages.h)."""
+    _fields_ = [
+        ("in", PagesState), ("out", PagesState),
+        ("rows", ct.c_int32), ("cap", ct.c_int32), ("n_pool", ct.c_int32), ("n_pools", ct.c_int32),
+        ("pools", ct.c_void_p * 128), ("page_bytes", ct.c_int64 * 128),
+        ("workspace", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+    ]
+
+
 EXPORTS = {
     "bmx_last_error": (ct.c_char_p, []),
     "bmx_k2b_page_bytes": (ct.c_size_t, [ct.POINTER(Geom)]),
@@ -338,6 +363,10 @@ EXPORTS = {
     "bmx_spectral_partial_count": (ct.c_int32, [ct.POINTER(SpectralDequantArgs)]),
     "bmx_fp16_decode_workspace_bytes": (ct.c_size_t, [ct.c_int, ct.c_int, ct.c_int]),
     "bmx_fp16_decode": (ct.c_int, [ct.POINTER(Fp16DecodeArgs), ct.c_void_p]),
+    "bmx_pages_update_workspace_bytes": (ct.c_size_t, [ct.POINTER(PagesUpdateArgs)]),
+    "bmx_pages_update": (ct.c_int, [ct.POINTER(PagesUpdateArgs), ct.c_void_p]),
+    "bmx_pages_compact_workspace_bytes": (ct.c_size_t, [ct.POINTER(PagesCompactArgs)]),
+    "bmx_pages_compact": (ct.c_int, [ct.POINTER(PagesCompactArgs), ct.c_void_p]),
     "bmx_prefill_workspace_bytes": (ct.c_size_t, [ct.POINTER(PrefillArgs)]),
     "bmx_prefill": (ct.c_int, [ct.POINTER(PrefillArgs), ct.c_void_p]),
 }

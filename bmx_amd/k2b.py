@@ -9,6 +9,7 @@ k2b decode path has no non-HIP fallback.
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -68,6 +69,18 @@ def _stream(dev: torch.device) -> ct.c_void_p:
     return ct.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def launch(fn, args, dev: torch.device, what: str) -> None:
+    """fn(args, stream) on dev's current stream, with dev the current device."""
+    index = dev.index
+    if index is not None and index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            rc = fn(ct.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        rc = fn(ct.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    if rc != 0:
+        _lib.check(rc, what)
+
+
 def _need(cond: bool, msg: str):
     if not cond:
         raise ValueError(msg)
@@ -114,6 +127,11 @@ def set_window_rows(a, B: int, h_kv: int, tail_len, tail_cap: int, new_kv=None) 
 
 def page_bytes(h_kv: int, rank: int, *, head_dim: int = HEAD_DIM, group: int = GROUP, k_bits: int = 3) -> int:
     return _lib.page_bytes(h_kv, rank, head_dim=head_dim, group=group, k_bits=k_bits)
+
+
+@functools.lru_cache(maxsize=None)
+def _page_bytes(h_kv: int, rank: int) -> int:   # of the recipe's page
+    return _lib.page_bytes(h_kv, rank)
 
 
 def geom(h_kv: int, rank: int, n_q_groups: int = 1, *, head_dim: int = HEAD_DIM, group: int = GROUP,
@@ -378,67 +396,63 @@ def decode_shared(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor
     >= tail_cap, 128) in q's dtype with tail_len rows (a device int32 (B,)
     tensor or a host int).  The recipe's page (128, 16 or 32, 64, 3).  A
     sequence that holds nothing gives zeros."""
-    _need(q.dim() == 4 and q.shape[3] == HEAD_DIM and q.dtype in (torch.float16, torch.bfloat16) and q.is_contiguous(),
-          "q must be contiguous fp16 or bf16 (B, h_kv, G, 128)")
+    _need(q.dim() == 4 and q.shape[3] == HEAD_DIM and (q.dtype is torch.float16 or q.dtype is torch.bfloat16)
+          and q.is_contiguous(), "q must be contiguous fp16 or bf16 (B, h_kv, G, 128)")
     B, h_kv, G, d = q.shape
-    dev = q.device
-    _need(q.is_cuda, "operands must be on a HIP device")
+    dev, on = q.device, q.get_device()
+    _need(on >= 0, "operands must be on a HIP device")
     _need(B > 0, "the batch is empty")
-    _need(consts.head_dim == d, "consts were made for another head_dim")
-    _need(pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous()
-          and pages.shape[1] == page_bytes(h_kv, rank), "pages must be a contiguous (n_pages, page_bytes) uint8 pool")
-    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
+    _need(len(consts.inv_freq) == d // 2, "consts were made for another head_dim")
+    _need(pages.dtype is torch.uint8 and pages.dim() == 2 and pages.is_contiguous()
+          and pages.shape[1] == _page_bytes(h_kv, rank), "pages must be a contiguous (n_pages, page_bytes) uint8 pool")
+    _need(page_table.dtype is torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
           and page_table.is_contiguous(), "page_table must be contiguous int32 (B, max_pages)")
-    _need(packed_len.dtype == torch.int32 and packed_len.numel() == B and packed_len.is_contiguous(),
+    _need(packed_len.dtype is torch.int32 and packed_len.numel() == B and packed_len.is_contiguous(),
           "packed_len must be int32[B]")
-    _need(basis16.shape == (h_kv * d, rank) and basis16.dtype == torch.float16 and basis16.is_contiguous(),
+    _need(basis16.shape == (h_kv * d, rank) and basis16.dtype is torch.float16 and basis16.is_contiguous(),
           "basis16 must be contiguous fp16 (C, rank)")
-    _need(rope.inv_freq == tuple(consts.inv_freq), "rope was made for other frequencies")
-    _need(rope.n_tokens >= max_packed_len, "rope holds fewer positions than max_packed_len")
-    tensors = [pages, page_table, packed_len, basis16, rope.data]
+    _need(rope.inv_freq is consts.inv_freq or rope.inv_freq == tuple(consts.inv_freq),
+          "rope was made for other frequencies")
+    table = rope.data
+    _need(table.shape[0] * PAGE_TOKENS >= max_packed_len, "rope holds fewer positions than max_packed_len")
     if out is None:
         out = torch.empty_like(q)
-    _need(out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous(),
-          "out must be contiguous and of q's shape and dtype")
-    a = _lib.DecodeSharedArgs()
-    a.geom = geom(h_kv, rank, G)
-    a.batch, a.io_dtype = B, _IO_DTYPES[q.dtype]
-    a.q, a.out = q.data_ptr(), out.data_ptr()
-    a.pages, a.n_pool_pages = pages.data_ptr(), pages.shape[0]
-    a.page_table, a.max_pages = page_table.data_ptr(), page_table.shape[1]
-    a.packed_len, a.max_packed_len, a.shared_len = packed_len.data_ptr(), int(max_packed_len), int(shared_len)
-    a.basis, a.rope, a.rope_pages = basis16.data_ptr(), rope.data.data_ptr(), rope.data.shape[0]
-    a.rope_scaling, a.sm_scale = consts.rope_scaling, float(sm_scale)
-    a.codebook[:] = consts.codebook
-    a.v_sign_bits[:] = consts.sign_bits
+    else:
+        _need(out.dtype is q.dtype and out.shape == q.shape and out.is_contiguous() and out.get_device() == on,
+              "out must be contiguous and of q's shape, dtype and device")
+    kt = vt = tl = None
+    sb = sh = st = tail_value = 0
     if tail_cap > 0:
         _need(k_tail is not None and v_tail is not None and k_tail.dim() == 4 and k_tail.shape == v_tail.shape
               and k_tail.stride() == v_tail.stride(), "k_tail/v_tail must share shape and strides")
-        _need(k_tail.dtype == q.dtype and v_tail.dtype == q.dtype and k_tail.shape[:2] == (B, h_kv)
+        _need(k_tail.dtype is q.dtype and v_tail.dtype is q.dtype and k_tail.shape[:2] == (B, h_kv)
               and k_tail.shape[2] >= tail_cap and k_tail.shape[3] == d and k_tail.stride(3) == 1,
               "k_tail/v_tail must be (B, h_kv, >=tail_cap, 128) in q's dtype with contiguous last dim")
-        a.k_tail, a.v_tail = k_tail.data_ptr(), v_tail.data_ptr()
+        _need(k_tail.get_device() == on and v_tail.get_device() == on, "operands must be on one device")
+        kt, vt = k_tail.data_ptr(), v_tail.data_ptr()
         # strides of size-1 dimensions are never used: taken as 0
-        a.tail_stride_b, a.tail_stride_h, a.tail_stride_t = (
-            0 if n == 1 else st for n, st in zip(k_tail.shape[:3], k_tail.stride()[:3]))
-        tensors += [k_tail, v_tail]
-    a.tail_cap = int(tail_cap)
+        sb, sh, st = (0 if n == 1 else x for n, x in zip(k_tail.shape[:3], k_tail.stride()[:3]))
     if isinstance(tail_len, torch.Tensor):
-        _need(tail_len.dtype == torch.int32 and tail_len.numel() == B and tail_len.is_contiguous(),
-              "tail_len must be a device int32[B] tensor or a host int")
-        a.tail_len = tail_len.data_ptr()
-        tensors.append(tail_len)
-    else:
-        a.tail_len_value = 0 if tail_len is None else int(tail_len)
-        _need(0 <= a.tail_len_value <= tail_cap, "tail_len must be within 0..tail_cap")
-    _need(all(t.device == dev for t in tensors) and out.device == dev, "operands must be on one device")
+        _need(tail_len.dtype is torch.int32 and tail_len.numel() == B and tail_len.is_contiguous()
+              and tail_len.get_device() == on, "tail_len must be a device int32[B] tensor or a host int")
+        tl = tail_len.data_ptr()
+    elif tail_len is not None:
+        tail_value = int(tail_len)
+        _need(0 <= tail_value <= tail_cap, "tail_len must be within 0..tail_cap")
+    _need(pages.get_device() == on and page_table.get_device() == on and packed_len.get_device() == on
+          and basis16.get_device() == on and table.get_device() == on, "operands must be on one device")
+    a = _lib.DecodeSharedArgs(
+        (h_kv, rank, G, d, GROUP, 3), B, _IO_DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), pages.data_ptr(),
+        pages.shape[0], page_table.shape[1], page_table.data_ptr(), packed_len.data_ptr(), int(max_packed_len),
+        int(shared_len), basis16.data_ptr(), table.data_ptr(), table.shape[0], consts.rope_scaling, float(sm_scale),
+        tuple(consts.codebook), tuple(consts.sign_bits), kt, vt, sb, sh, st, tl, tail_value, int(tail_cap))
     lib = _lib.lib()
-    with torch.cuda.device(dev):
-        # scratch of the call's own, from torch's allocator: calls on two streams or in two graphs share none
-        need = int(lib.bmx_k2b_decode_shared_workspace_bytes(ct.byref(a)))
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    # scratch of the call's own, from torch's allocator: calls on two streams or in two graphs share none
+    need = int(lib.bmx_k2b_decode_shared_workspace_bytes(ct.byref(a)))
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        _lib.check(lib.bmx_k2b_decode_shared(ct.byref(a), _stream(dev)), "bmx_k2b_decode_shared")
+    launch(lib.bmx_k2b_decode_shared, a, dev, "bmx_k2b_decode_shared")
     return out
 
 

@@ -19,7 +19,7 @@ import ctypes as ct
 import torch
 
 from . import _lib
-from .k2b import DecodeWorkspace, _need, _stream
+from .k2b import DecodeWorkspace, _need, _stream, launch
 
 HEAD_DIM = 128
 DTYPES = {torch.float16: 0, torch.bfloat16: 1}   # BMX_PREFILL_F16 / BF16
@@ -69,22 +69,18 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     if out is None:
         out = torch.empty(hq, n_q, HEAD_DIM, dtype=q.dtype, device=q.device)
     _need(out.shape == (hq, n_q, HEAD_DIM) and out.dtype == q.dtype and out.is_contiguous(), "out (Hq, n_q, 128)")
-    a = _lib.PrefillArgs()
-    a.q, a.q_stride_h, a.q_stride_t = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.v, a.kv_stride_h, a.kv_stride_t = k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)
-    a.out = out.data_ptr()
-    a.h_kv, a.n_q_groups, a.n_q, a.n_kv = h_kv, hq // h_kv, n_q, n_kv
-    a.head_dim, a.dtype, a.causal, a.sm_scale = HEAD_DIM, DTYPES[q.dtype], int(bool(causal)), float(scale)
-    a.n_split = int(n_split)
-    a.window, a.sinks = window, sinks
+    qh, qt, _ = q.stride()
+    kh, kt, _ = k.stride()
+    a = _lib.PrefillArgs(q.data_ptr(), qh, qt, k.data_ptr(), v.data_ptr(), kh, kt, out.data_ptr(), h_kv, hq // h_kv,
+                         n_q, n_kv, HEAD_DIM, DTYPES[q.dtype], int(bool(causal)), float(scale), int(n_split), None, 0,
+                         window, sinks)
     L = _lib.lib()
     if window:   # scratch of its own, from torch's allocator: calls on two streams or in two graphs share none
-        with torch.cuda.device(q.device):
-            need = int(L.bmx_prefill_workspace_bytes(ct.byref(a)))
-            if need:
-                ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), need
-            _lib.check(L.bmx_prefill(ct.byref(a), _stream(q.device)), "bmx_prefill")
+        need = int(L.bmx_prefill_workspace_bytes(ct.byref(a)))
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        launch(L.bmx_prefill, a, q.device, "bmx_prefill")
         return out
     need = int(L.bmx_prefill_workspace_bytes(ct.byref(a)))
     if need:
