@@ -138,7 +138,8 @@ def packed_attention_forward(module, query, key, value, attention_mask, scaling,
         raise NotImplementedError("the packed cache serves batch size 1")
     q = query.squeeze(0)
     n_q = q.shape[1]
-    out = module._packed_layer.attend(q, scaling, is_causal=n_q > 1, attention_mask=attention_mask)
+    out = module._packed_layer.attend(q, scaling, is_causal=n_q > 1, attention_mask=attention_mask,
+                                      sliding_window=kwargs.get("sliding_window"))
     n_h, n_q, d = out.shape
     return out.transpose(0, 1).reshape(1, n_q, n_h * d).to(query.dtype), None
 
@@ -533,8 +534,10 @@ class PackedStreamingLayer(DynamicLayer):
     # -------------------------------------------------------------- read side
 
     def attend(self, q: torch.Tensor, scaling: float, is_causal: bool = False,
-               attention_mask: torch.Tensor | None = None) -> torch.Tensor:
-        """q (n_q_heads, n_q, d) post-RoPE -> (n_q_heads, n_q, d)."""
+               attention_mask: torch.Tensor | None = None, sliding_window: int | None = None) -> torch.Tensor:
+        """q (n_q_heads, n_q, d) post-RoPE -> (n_q_heads, n_q, d).  sliding_window:
+        the model layer's (HF hands it over beside the mask); a prefill whose
+        mask it is needs no mask tensor."""
         if q.device.type != "cuda":
             raise RuntimeError("the packed cache attends on a HIP device only (no CPU path)")
         n_heads, n_q, d = q.shape
@@ -543,7 +546,7 @@ class PackedStreamingLayer(DynamicLayer):
             if self._path == "spectral":
                 return self._decode_spectral(q, scaling, G)
             return self._decode(q, scaling, G)
-        return self._dense(q, scaling, G, is_causal and n_q > 1, attention_mask)
+        return self._dense(q, scaling, G, is_causal and n_q > 1, attention_mask, sliding_window)
 
     def _decode(self, q: torch.Tensor, scaling: float, G: int) -> torch.Tensor:
         """One query step through the layer's bound decode plan: q, the window
@@ -624,7 +627,7 @@ class PackedStreamingLayer(DynamicLayer):
                                         k_win=kw, v_win=vw, apply_rope=k2b.ROPE_FP16_TABLES)
         return out.reshape(h * G, 1, d)
 
-    def _dense(self, q, scaling, G, causal, attention_mask):
+    def _dense(self, q, scaling, G, causal, attention_mask, sliding_window=None):
         """Prefill (n_q > 1): _prefill_dense_attention (chunked_attention.py:
         320-395).  The page kernel dequantizes the committed pages straight to
         the model dtype (k2b keys rotated in the same pass with the fp16 RoPE
@@ -632,7 +635,8 @@ class PackedStreamingLayer(DynamicLayer):
         call reads the grouped heads in place (no G-fold copy of K and V).
         With no mask, or fewer queries than keys and the model's mask equal to
         the causal mask of the last n_q positions (bottom right), that is
-        bmx_prefill (fp16 / bf16, head dim 128); other head dims take SDPA's
+        bmx_prefill (fp16 / bf16, head dim 128), and so is the causal mask
+        within the layer's sliding window; other head dims take SDPA's
         flash kernel or its bottom-right causal bias for the same masks; any
         other mask takes SDPA's memory-efficient kernel over expanded heads."""
         dev, dt = q.device, q.dtype
@@ -667,6 +671,8 @@ class PackedStreamingLayer(DynamicLayer):
             # bmx_prefill: grouped heads read their K/V head in place; causal
             # is the bottom-right mask (n_q == n_kv: the ordinary one)
             return prefill.attention(q, Kd, Vd, scaling, causal=causal or lower_right)
+        if _is_window_mask(attention_mask, n_q, n_kv, sliding_window) and prefill.supported(q, Kd, Vd):
+            return prefill.attention(q, Kd, Vd, scaling, causal=True, window=sliding_window)
         if lower_right:
             # the queries are the last n_q positions: causal from the bottom
             # right, which ROCm's kernels take as a bias of their own (grouped
@@ -707,6 +713,17 @@ def _is_lower_right_causal(mask, n_q: int, n_kv: int) -> bool:
     answer = bool(torch.equal(mask[0, 0], j <= i + (n_kv - n_q)))
     _MASK_SEEN[:] = [weakref.ref(mask), mask._version, answer]
     return answer
+
+
+def _is_window_mask(mask, n_q: int, n_kv: int, window: int | None) -> bool:
+    """Whether a model's boolean mask (1, 1, n_q, n_kv) is exactly the causal
+    mask of the last n_q positions within a sliding window: one device compare
+    (the host waits for it)."""
+    if not window or window < 1 or mask is None or mask.dtype != torch.bool or mask.dim() != 4 or n_q > n_kv \
+            or tuple(mask.shape) != (1, 1, n_q, n_kv):
+        return False
+    gap = torch.arange(n_q, device=mask.device)[:, None] + (n_kv - n_q) - torch.arange(n_kv, device=mask.device)[None, :]
+    return bool(torch.equal(mask[0, 0], (gap >= 0) & (gap < window)))
 
 
 # ------------------------------------------------------------------ cache
@@ -904,7 +921,7 @@ class StreamingQuantizedLayer(PackedStreamingLayer):
         S = self._committed_S_q + self._T
         self.keys, self.values = self._slab_k[:, :, :S], self._slab_v[:, :, :S]
 
-    def attend(self, q, scaling, is_causal=False, attention_mask=None):
+    def attend(self, q, scaling, is_causal=False, attention_mask=None, sliding_window=None):
         raise RuntimeError("StreamingQuantizedLayer is read by the model's own attention")
 
 

@@ -93,25 +93,25 @@ __device__ __forceinline__ int block_scan(int v, int* s_tmp, int& total) {
   return before + x - v;
 }
 
-// grid (x: 1024-entry pieces of a row, or of the refs in the last y; y: new rows, then the refs)
+// workgroups 0 .. new_rows * pieces - 1: 1024 entries of a new row; then 1024 refs each
 __global__ __launch_bounds__(kPgThreads) void rows_kernel(const UpdateArgs a) {
-  const int i = blockIdx.y;
-  const int64_t e0 = (int64_t)blockIdx.x * kPgChunk + threadIdx.x;
-  if (i == a.new_rows) {
+  const int pieces = (a.cap + kPgChunk - 1) / kPgChunk, i = (int)blockIdx.x / pieces;
+  if (i >= a.new_rows) {
+    const int p0 = ((int)blockIdx.x - a.new_rows * pieces) * kPgChunk + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t p = e0 + u * kPgThreads;
+      const int p = p0 + u * kPgThreads;
       if (p < a.n_pool) a.out.refs[p] = a.in.refs[p];
     }
     return;
   }
-  if ((int64_t)blockIdx.x * kPgChunk >= a.cap) return;
+  const int piece = (int)blockIdx.x - i * pieces;
   const int src = source_row(a, i);
   const int len = src < 0 ? 0 : row_len(a.in, src, a.cap);
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.lens[i] = len;
+  if (piece == 0 && threadIdx.x == 0) a.lens[i] = len;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const int64_t e = e0 + u * kPgThreads;
+    const int e = piece * kPgChunk + threadIdx.x + u * kPgThreads;
     if (e < a.cap) a.out.table[(int64_t)i * a.cap + e] = e < len ? a.in.table[(int64_t)src * a.cap + e] : 0;
   }
 }
@@ -558,8 +558,9 @@ extern "C" int bmx_pages_update(const bmx_pages_update_args* a, void* stream) {
   const size_t lds = 2 * (size_t)a->new_rows * sizeof(int);
   if (lds > 48 * 1024 && bmx_ensure_dynamic_lds((const void*)stack_kernel, lds) != hipSuccess)
     return pg_fail(name, BMX_PAGES_E_HIP, "too many rows for the device's LDS");
-  hipLaunchKernelGGL(rows_kernel, dim3(std::max(pieces, (unsigned)k.chunks), (unsigned)a->new_rows + 1),
-                     dim3(kPgThreads), 0, st, k);
+  const int64_t row_wgs = (int64_t)a->new_rows * pieces + k.chunks;
+  if (row_wgs > INT32_MAX) return pg_fail(name, BMX_PAGES_E_INVALID, "too many table entries");
+  hipLaunchKernelGGL(rows_kernel, dim3((unsigned)row_wgs), dim3(kPgThreads), 0, st, k);
   if (a->index) {
     hipLaunchKernelGGL(count_kernel, dim3(pieces, (unsigned)a->rows), dim3(kPgThreads), 0, st, k);
     hipLaunchKernelGGL(freed_kernel, dim3((unsigned)k.chunks), dim3(kPgThreads), 0, st, k);

@@ -1,7 +1,7 @@
 """The decode-path calls as ``torch.library`` custom operators.
 
-``torch.ops.bmx.k2b_decode`` / ``k2b_append`` / ``rtn_decode`` / ``rtn_append``
-are the same C-ABI calls as ``bmx_amd.k2b`` / ``bmx_amd.rtn`` (one ctypes call
+``torch.ops.bmx.k2b_decode`` / ``k2b_decode_shared`` / ``k2b_append`` /
+``rtn_decode`` / ``rtn_append`` are the same C-ABI calls as ``bmx_amd.k2b`` / ``bmx_amd.rtn`` (one ctypes call
 each on the current stream), and ``torch.ops.bmx.prefill_attention`` the
 prefill attention of ``bmx_amd.prefill`` (chunked_attention.py:320-395 calls
 SDPA there), registered so that the dispatcher, FakeTensor
@@ -62,6 +62,28 @@ def _(q, pages, page_table, packed_len, max_packed_len, basis16, inv_freq, rope_
     return torch.empty_like(q)
 
 
+@torch.library.custom_op(f"{_LIB}::k2b_decode_shared", mutates_args=(), device_types="cuda")
+def k2b_decode_shared(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, packed_len: torch.Tensor,
+                      max_packed_len: int, shared_len: int, basis16: torch.Tensor, rope: torch.Tensor,
+                      inv_freq: list[float], rope_scaling: float, codebook: list[float], sign_bits: list[int],
+                      sm_scale: float, rank: int, k_tail: Optional[torch.Tensor] = None,
+                      v_tail: Optional[torch.Tensor] = None, tail_len: Optional[torch.Tensor] = None,
+                      tail_len_value: int = 0, tail_cap: int = 0) -> torch.Tensor:
+    """One decode step of a batch behind a common prefix
+    (``bmx_amd.k2b.decode_shared``; rope: a ``RopeTable``'s data)."""
+    consts = _consts(inv_freq, rope_scaling, codebook, sign_bits)
+    return k2b.decode_shared(q, pages, page_table, packed_len, max_packed_len, shared_len, basis16, consts, sm_scale,
+                             rank=rank, rope=k2b.RopeTable(rope, consts.inv_freq), k_tail=k_tail, v_tail=v_tail,
+                             tail_len=_tail_len(tail_len, tail_len_value), tail_cap=tail_cap)
+
+
+@k2b_decode_shared.register_fake
+def _(q, pages, page_table, packed_len, max_packed_len, shared_len, basis16, rope, inv_freq, rope_scaling, codebook,
+      sign_bits, sm_scale, rank, k_tail=None, v_tail=None, tail_len=None, tail_len_value=0, tail_cap=0):
+    torch._check(q.dim() == 4 and q.shape[-1] == k2b.HEAD_DIM)
+    return torch.empty_like(q)
+
+
 @torch.library.custom_op(f"{_LIB}::k2b_append", mutates_args=("pages",), device_types="cuda")
 def k2b_append(k_pre: torch.Tensor, v: torch.Tensor, basis32: torch.Tensor, basis16: torch.Tensor,
                pages: torch.Tensor, page_ids: torch.Tensor, codebook: list[float], sign_bits: list[int],
@@ -114,15 +136,15 @@ def _(k, v, pages, page_ids, k_bits, v_bits, k_group, v_group, k_arm=rtn.TOKEN):
 
 @torch.library.custom_op(f"{_LIB}::prefill_attention", mutates_args=(), device_types="cuda")
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, causal: bool,
-                      n_split: int = 0) -> torch.Tensor:
+                      n_split: int = 0, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """Attention of (h_kv * G, n_q, 128) queries over (h_kv, n_kv, 128) K/V
-    rows, grouped heads, bottom-right causal or no mask
-    (``bmx_amd.prefill.attention``)."""
-    return prefill.attention(q, k, v, sm_scale, causal=causal, n_split=n_split)
+    rows, grouped heads, bottom-right causal (within a sliding window, with
+    sinks) or no mask (``bmx_amd.prefill.attention``)."""
+    return prefill.attention(q, k, v, sm_scale, causal=causal, n_split=n_split, window=window, sinks=sinks)
 
 
 @prefill_attention.register_fake
-def _(q, k, v, sm_scale, causal, n_split=0):
+def _(q, k, v, sm_scale, causal, n_split=0, window=0, sinks=0):
     torch._check(q.dim() == 3 and q.shape[-1] == prefill.HEAD_DIM and k.dim() == 3)
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
