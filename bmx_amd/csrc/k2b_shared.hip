@@ -33,9 +33,12 @@
 // both buffers in LDS are double, and the values of a tile are added during the
 // keys and scores of the next (their products and table reads fill the gaps of
 // its vector work).
-// Rounded to 16 bits: K once (its low-rank part, residual and rotation are fp32
-// on fp16 factors), the rotations, x, and Q when bf16 (by a power of two).  Every
-// sum, c and l are fp32.
+// Rounded to 16 bits: x, Q when bf16 (by a power of two), and K when bf16.  With
+// fp16 queries a rebuilt key stays in two fp16 parts, each with a score product:
+// one part left the output 2.4 times as far from 64-bit values as its own rounding
+// does (rms), two leave 1.4 times, for 10% of the time.  The rotations come in
+// 16-bit fixed point, as wide as fp16 and 16 times as close.  Every sum, c and l
+// are fp32.
 // A workgroup leaves one fp32 partial a row, and shared_merge_kernel joins a row's
 // partials, un-rotates the packed ones (H128, signs) and adds the window's.
 
@@ -81,17 +84,29 @@ struct SharedArgs {
   float* part;                     // [B][h_kv][G][n_slots][kShPitch]
 };
 
-// One key pair (j, j + 64): low-rank part plus residual code times scale,
-// rotated by packed (cos, sin): (k_j c - k_{j+64} s, k_{j+64} c + k_j s).
-__device__ __forceinline__ half2_t key_pair(float lo, float hi, half2_t code, half2_t scale, half2_t cs) {
-  lo = __builtin_fmaf((float)code[0], (float)scale[0], lo);
-  hi = __builtin_fmaf((float)code[1], (float)scale[1], hi);
-  // x times a half of cs in one instruction (the compiler converts the half first)
-  float lc, hc;
-  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(lc) : "v"(lo), "v"(as_u32(cs)));
-  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(hc) : "v"(hi), "v"(as_u32(cs)));
-  const float s = (float)cs[1];
-  return half2_t{(_Float16)__builtin_fmaf(-hi, s, lc), (_Float16)__builtin_fmaf(lo, s, hc)};
+// One key pair (j, j + 64): low-rank part plus residual code times scale, rotated,
+// (k_j c - k_{j+64} s, k_{j+64} c + k_j s) in fp32 with c, s times kRopeOne, as
+// fp16 k and, where kLow, the fp16 rest (together 2^-22 of a key)
+constexpr float kRopeOne = 32767.0f;   // 1 in the rotation table's 16-bit fixed point
+template <bool kLow>
+__device__ __forceinline__ void key_pair(float lo, float hi, half2_t code, half2_t scale, uint32_t cs, half2_t& k,
+                                         half2_t& low) {
+  const float a = __builtin_fmaf((float)code[0], (float)scale[0], lo);
+  const float b = __builtin_fmaf((float)code[1], (float)scale[1], hi);
+  const float c = (float)(int16_t)(cs & 0xffff), s = (float)(int16_t)(cs >> 16);
+  const float u = __builtin_fmaf(-b, s, a * c), v = __builtin_fmaf(a, s, b * c), unit = 1.0f / kRopeOne;
+  // one instruction a half: the product with 1 / kRopeOne, rounded, then what that left
+  uint32_t d;
+  asm("v_fma_mixlo_f16 %0, %1, %3, 0\n\tv_fma_mixhi_f16 %0, %2, %3, 0" : "=&v"(d) : "v"(u), "v"(v), "s"(unit));
+  k = as_h2(d);
+  if constexpr (kLow) {
+    uint32_t e;
+    asm("v_fma_mixlo_f16 %0, %2, %4, -%1 op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %0, %3, %4, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+        : "=&v"(e)
+        : "v"(d), "v"(u), "v"(v), "s"(unit));
+    low = as_h2(e);
+  }
 }
 
 constexpr int kTilePages = kShWaves;   // a page a wave
@@ -120,6 +135,7 @@ __device__ __forceinline__ void packed_rows(const SharedArgs& a, uint8_t* smem, 
                                             const int32_t* ptab, int g0, int g1, int slot, Limit limit) {
   constexpr int KQ = R / 4;   // rank elements of a lane in the key product
   typedef _Float16 hvec_t __attribute__((ext_vector_type(KQ)));
+  constexpr bool kLow = DT == BMX_PREFILL_F16;   // keys in two fp16 parts (bf16's own rounding hides the second)
   using Lds = ShLds<R, NR>;
   uint2* vlut = reinterpret_cast<uint2*>(smem + Lds::kVlut);
   hvec_t* s_basis = reinterpret_cast<hvec_t*>(smem + Lds::kBasis);
@@ -341,21 +357,22 @@ __device__ __forceinline__ void packed_rows(const SharedArgs& a, uint8_t* smem, 
         khi = __builtin_amdgcn_mfma_f32_16x16x16f16(bhi, us, z, 0, 0, 0);
       }
       if constexpr (!kFirst) values(t - 1, bb);
-      const u32x4_t cv = cs[bb & 1];
       const uint4 s4 = *reinterpret_cast<const uint4*>(s_scale + wave * 64 + 16 * bb + 4 * q);
       const half2_t sc[4] = {as_h2(s4.x), as_h2(s4.y), as_h2(s4.z), as_h2(s4.w)};
       const half2_t cp[4] = {kres_pair<4 * bb + 0>(km, kres[0], kres[1], kres[2]),
                              kres_pair<4 * bb + 1>(km, kres[0], kres[1], kres[2]),
                              kres_pair<4 * bb + 2>(km, kres[0], kres[1], kres[2]),
                              kres_pair<4 * bb + 3>(km, kres[0], kres[1], kres[2])};
-      union { half2_t h2[4]; half8_t v; } ka;
+      union { half2_t h2[4]; half8_t v; } ka, kb;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ka.h2[i] = key_pair(klo[i], khi[i], cp[i], sc[i], as_h2(cv[i]));
+      for (int i = 0; i < 4; ++i) key_pair<kLow>(klo[i], khi[i], cp[i], sc[i], cs[bb & 1][i], ka.h2[i], kb.h2[i]);
       if constexpr (bb < 2) cs[bb & 1] = __builtin_amdgcn_raw_buffer_load_b128(rope, lane * 16, (bb + 2) * 1024, 0);
 #pragma unroll
-      for (int rb = 0; rb < NR; ++rb)
-        s[rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            ka.v, __builtin_bit_cast(half8_t, s_q[(rb * 4 + bb) * 64 + lane]), s[rb], 0, 0, 0);
+      for (int rb = 0; rb < NR; ++rb) {
+        const half8_t qv = __builtin_bit_cast(half8_t, s_q[(rb * 4 + bb) * 64 + lane]);
+        s[rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka.v, qv, s[rb], 0, 0, 0);
+        if constexpr (kLow) s[rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb.v, qv, s[rb], 0, 0, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
     slice(std::integral_constant<int, 0>{});
@@ -687,12 +704,11 @@ __global__ __launch_bounds__(64) void rope_table_kernel(const RopeArgs a) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float sn, cs;
-      sincosf(a.inv_freq[16 * b + 4 * q + i] * pos, &sn, &cs);
-      const half2_t v = {(_Float16)cs, (_Float16)sn};
-      w[i] = as_u32(v);
+      float s, c;
+      sincosf(a.inv_freq[16 * b + 4 * q + i] * pos, &s, &c);
+      w[i] = (uint32_t)(uint16_t)__float2int_rn(kRopeOne * c) | (uint32_t)__float2int_rn(kRopeOne * s) << 16;
     }
-    *reinterpret_cast<uint4*>(a.out + ((int64_t)blockIdx.x * 4 + b) * 256 + lane * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(a.out)[((int64_t)blockIdx.x * 4 + b) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 

@@ -229,9 +229,10 @@ int bmx_k2b_decode_noalloc(const bmx_k2b_decode_args* args, void* stream);
  * ---------------------------------------------------------------------- */
 
 /* Rotation table of positions 0 .. 16 n_pages - 1, read by the shared-prefix
- * decode of every layer: fp16 (cos, sin) of HF's angle fl32(inv_freq_j * pos),
- * without rope_scaling, 4096 bytes a page: [page][b][lane 16q+n][i] holds
- * token n, pair j = 16b + 4q + i (b, i < 4).  Written once a model. */
+ * decode of every layer: cos and sin of HF's angle fl32(inv_freq_j * pos),
+ * without rope_scaling, as int16 round(32767 x) (off by 2^-16 at most, where fp16
+ * would be by 2^-12), 4096 bytes a page: [page][b][lane 16q+n][i] holds token n's
+ * (cos, sin) of pair j = 16b + 4q + i (b, i < 4).  Written once a model. */
 #define BMX_K2B_ROPE_PAGE_BYTES 4096
 int bmx_k2b_rope_table(const float inv_freq[64], int32_t n_pages, void* out, void* stream);
 
