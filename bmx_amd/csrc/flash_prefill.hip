@@ -483,11 +483,13 @@ std::string pf_check(const bmx_prefill_args* a) {
   if (a->window < 0 || a->sinks < 0) return "window and sinks must be >= 0";
   if (a->sinks > 0 && a->window == 0) return "sinks need a window";
   if (a->window > 0 && !a->causal) return "a window needs causal";
+  if (a->window > 0 && ((uintptr_t)a->workspace & 15)) return "workspace must be 16-byte aligned";
   return "";
 }
 
-// a window that hides some key from some row (one as long as the keys hides none)
-bool pf_windowed(const bmx_prefill_args* a) { return a->window > 0 && a->window < a->n_kv; }
+// the window form, also where the window is as long as the keys: its rows keep
+// clear of infinite and NaN values that the causal mask hides from them
+bool pf_windowed(const bmx_prefill_args* a) { return a->window > 0; }
 // the window form of few rows (prefill_rows.hip)
 bool pf_few_rows(const bmx_prefill_args* a) {
   return a->window > 0 && (int64_t)a->n_q * a->n_q_groups <= kRowsMax;

@@ -29,7 +29,7 @@
 // With the sums spread over the waves by channels a wave keeps 4 NR registers of
 // them, and 128 registers in all let two workgroups share a CU (a form with a
 // wave's own tiles and all channels kept 32 NR, spilled, and took 177 us where
-// this takes 65, at 64k tokens and 16 sequences of up to 1,024 more).  One barrier a tile:
+// this took 65, at 64k tokens and 16 sequences of up to 1,024 more).  One barrier a tile:
 // both buffers in LDS are double, and the values of a tile are added during the
 // keys and scores of the next (their products and table reads fill the gaps of
 // its vector work).
@@ -39,6 +39,8 @@
 // does (rms), two leave 1.4 times, for 10% of the time.  The rotations come in
 // 16-bit fixed point, as wide as fp16 and 16 times as close.  Every sum, c and l
 // are fp32.
+// Vector instructions bound it: at 64k tokens and 16 sequences (73 us) they are
+// active in 71% of the cycles, matrix products in 24%, LDS in 38%.
 // A workgroup leaves one fp32 partial a row, and shared_merge_kernel joins a row's
 // partials, un-rotates the packed ones (H128, signs) and adds the window's.
 
@@ -763,11 +765,11 @@ struct SharedPlan {
 
 // Row blocks of 16, 32 or 64 rows.  The prefix is split over one workgroup a CU,
 // over two (as many as fit) where each still walks 6 tiles, and over no more than
-// it has tiles: at 16 sequences, G 4, h_kv 8, 64k tokens take 58.9 us with one a
-// CU (16 tiles each) and 51.9 with two (8), 16k tokens 26.8 (4) and 30.0 (2).  A
-// sequence's own pages go over workgroups of 8 groups (4 tiles): 1,024 tokens each
-// behind 64k 58.5 us, with 16 groups 63.7, with 4 62.5; longer ones where there
-// would be over 2048.
+// it has tiles: at 16 sequences, G 4, h_kv 8, 64k tokens take 69 us with one a CU
+// (16 tiles each) and 60 with two (8), 16k tokens 29 (4) and 32 (2).  A sequence's
+// own pages go over workgroups of 8 groups (4 tiles): 1,024 tokens each behind 64k
+// 73 us, with 4 groups 74; without a prefix 8 groups 19, 4 groups 18, 2 groups 23;
+// longer ones where there would be over 2048.
 SharedPlan sh_plan(const bmx_k2b_decode_shared_args* a) {
   SharedPlan p{};
   const int h = a->geom.h_kv, rows = a->batch * a->geom.n_q_groups, cus = bmx_device_cu_count();

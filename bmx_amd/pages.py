@@ -35,7 +35,7 @@ class PageState:
     its pages in order; refs (n_pool,), the uses of each page (a table entry is
     one; a holder outside the tables adds its own); free (n_pool,), a stack of
     n_free[0] free ids, the top at its end; status (1,) of the update that made
-    the state (compact leaves it)."""
+    the state (compact leaves it; None in a new state of compact's)."""
 
     table: torch.Tensor
     n_pages: torch.Tensor
@@ -84,8 +84,6 @@ def _out(state: PageState, out: PageState | None, rows: int, on: int) -> PageSta
         return state.like(rows)
     _need(_check(out, "out") == on and out.table.shape == (rows, state.table.shape[1])
           and out.refs.shape == state.refs.shape, "out: a state of the new rows over the same pool")
-    if out.status is None:
-        out.status = out.n_free.new_empty(1)
     return out
 
 
@@ -108,10 +106,15 @@ def update(state: PageState, index: torch.Tensor | None = None, grow: torch.Tens
         rows = index.shape[0]
     _need(grow is None or grow.shape[0] == rows, "grow: one count a new row")
     o = _out(state, out, rows, on)
+    if o.status is None:
+        o.status = o.n_free.new_empty(1)
+    st = o.status
+    _need(st.dtype is torch.int32 and st.numel() == 1 and st.get_device() == on,
+          "out: status, one int32 on the state's device")
     dev = state.table.device
     a = _lib.PagesUpdateArgs(_ptrs(state), _ptrs(o), old, rows, cap, state.refs.shape[0],
                              None if index is None else index.data_ptr(), None if grow is None else grow.data_ptr(),
-                             o.status.data_ptr())
+                             st.data_ptr())
     lib = _lib.lib()
     need = int(lib.bmx_pages_update_workspace_bytes(ct.byref(a)))
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
@@ -124,7 +127,9 @@ def compact(state: PageState, pools, *, out: PageState | None = None) -> PageSta
     """The state with its n live pages (refs > 0) at ids below n: those above
     move, lowest first, to the free ids below, in every pool of ``pools`` (uint8
     (n_pool, page_bytes) tensors, page sizes multiples of 16, changed in place).
-    The free stack then hands out the lowest id first."""
+    The free stack then hands out the lowest id first.  A holder outside the
+    tables is not told its pages' new ids: one that reads them keeps them as a
+    row of the table."""
     on = _check(state, "state")
     n_pool, dev = state.refs.shape[0], state.table.device
     pools = list(pools)
@@ -134,6 +139,8 @@ def compact(state: PageState, pools, *, out: PageState | None = None) -> PageSta
               and p.get_device() == on, "pools: contiguous uint8 (n_pool, page_bytes) on the state's device")
         _need(p.shape[1] % 16 == 0 and p.shape[1] > 0, "pools: page_bytes must be a multiple of 16")
     o = _out(state, out, state.table.shape[0], on)
+    if out is None:
+        o.status = None
     a = _lib.PagesCompactArgs(_ptrs(state), _ptrs(o), *state.table.shape, n_pool, len(pools))
     for i, p in enumerate(pools):
         a.pools[i], a.page_bytes[i] = p.data_ptr(), p.shape[1]

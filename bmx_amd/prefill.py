@@ -48,7 +48,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     ``h``.  With ``causal`` query i sees keys ``j <= p = i + n_kv - n_q``; with
     ``window`` > 0 as well only those with ``j > p - window`` (HF's
     sliding_window: the query's own key is one of the window) or ``j < sinks``.
-    Rows that no query sees may hold anything.  Few rows (n_q * G up to 16, a
+    Under a window, rows that a query does not see may hold anything (infinities
+    and NaN among it) and do not reach its output.  Few rows (n_q * G up to 16, a
     token's attention) under a window run on a form of their own, the keys
     spread over the chip.
     Returns (h_kv * G, n_q, 128) in q's dtype, contiguous."""
@@ -68,7 +69,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     window, sinks = min(window, 2**31 - 1), min(sinks, 2**31 - 1)
     if out is None:
         out = torch.empty(hq, n_q, HEAD_DIM, dtype=q.dtype, device=q.device)
-    _need(out.shape == (hq, n_q, HEAD_DIM) and out.dtype == q.dtype and out.is_contiguous(), "out (Hq, n_q, 128)")
+    _need(out.shape == (hq, n_q, HEAD_DIM) and out.dtype == q.dtype and out.is_contiguous()
+          and out.device == q.device, "out (Hq, n_q, 128)")
     qh, qt, _ = q.stride()
     kh, kt, _ = k.stride()
     a = _lib.PrefillArgs(q.data_ptr(), qh, qt, k.data_ptr(), v.data_ptr(), kh, kt, out.data_ptr(), h_kv, hq // h_kv,

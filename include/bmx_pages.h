@@ -66,7 +66,8 @@ int bmx_pages_update(const bmx_pages_update_args* a, void* stream);
 // With n live pages (refs > 0), those at ids n and up move to the free ids below
 // n, lowest to lowest, in every pool; tables, refs and the stack follow (the
 // stack hands out the lowest id first).  What a page left behind stays as it
-// was.  The pools are changed in place.
+// was.  The pools are changed in place.  A holder outside the tables is not told
+// its pages' new ids: one that reads them keeps them as a row of the table.
 typedef struct bmx_pages_compact_args {
   bmx_pages_state in, out;
   int32_t rows, cap, n_pool;

@@ -48,7 +48,8 @@ typedef struct bmx_prefill_args {
   size_t workspace_bytes;
   int window;             // > 0 (needs causal): query i, at position p = i + n_kv - n_q, sees keys
                           // p - window < j <= p and the sinks; 0: no window.  K and V rows that no
-                          // query sees may hold anything, infinities and NaN among it
+                          // query sees may hold anything, infinities and NaN among it, and those
+                          // that a query does not see do not reach its output
   int sinks;              // first keys that every query at or past them sees (needs a window); 0: none
 } bmx_prefill_args;
 

@@ -297,3 +297,24 @@ def test_a_served_batch_from_prompt_to_compaction():
     t = pages.compact(pages.update(t, _dev([1]), None), [pool])
     assert t.n_free.item() == 200 - 48 and t.table[0, :48].max().item() == 47
     assert torch.equal(attend(t, [0]), before[1:])
+
+
+def test_status_belongs_to_updates():
+    """compact's new state has no status, buffers given to it keep theirs, and an
+    update makes or checks one."""
+    s = pages.PageState.make(2, 8, 16, DEV)
+    s = pages.update(s, None, _dev([3, 2]))
+    c = pages.compact(s, [])
+    assert c.status is None
+    buf = s.like()
+    buf.status.fill_(7)
+    pages.compact(s, [], out=buf)
+    assert buf.status.item() == 7
+    nxt = pages.update(c, _dev([1, 0]), out=c.like())
+    assert nxt.status.item() == pages.OK and nxt.n_pages.tolist() == [2, 3]
+    bare = c.like()
+    bare.status = None
+    assert pages.update(c, None, out=bare).status.item() == pages.OK
+    bare.status = torch.zeros(1, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="status"):
+        pages.update(c, None, out=bare)

@@ -166,6 +166,24 @@ def test_infinite_value_reaches_only_the_rows_that_see_it(G, n_q, dtype):
         assert ((out[h][rows].double() - ref[rows]).abs() <= u * (ref[rows].abs() + 5.0) + 1e-4).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [500, 100000])
+@pytest.mark.parametrize("G,n_q", [(2, 200), (2, 4)])
+def test_window_as_long_as_the_keys_keeps_hidden_values_out(G, n_q, window, dtype):
+    """Nothing but the causal mask hides a key: a NaN value reaches the rows from
+    its own on, and the rows before are those of the call without it."""
+    n_kv = 500
+    q, k, v = _inputs(1, G, n_q, n_kv, dtype, seed=8)
+    clean = prefill.attention(q, k, v, SCALE, causal=True, window=window)
+    row = n_q // 2
+    v[0, n_kv - n_q + row, 77] = float("nan")
+    out = prefill.attention(q, k, v, SCALE, causal=True, window=window)
+    torch.cuda.synchronize()
+    assert torch.equal(out[:, :row], clean[:, :row])
+    assert torch.isnan(out[:, row:, 77]).all()
+    assert torch.isfinite(out[:, row:, :77]).all() and torch.isfinite(out[:, row:, 78:]).all()
+
+
 def test_repeated_calls_are_equal_bit_for_bit():
     for n_q in (1, 64):
         q, k, v = _inputs(4, 4, n_q, 3000, torch.float16, seed=9)

@@ -46,3 +46,11 @@ def test_wrapper_refuses_cpu_tensors_and_bad_arguments():
     q, k = torch.zeros(4, 1, 128, dtype=torch.float16), torch.zeros(1, 8, 128, dtype=torch.float16)
     with pytest.raises(ValueError, match="HIP device"):
         prefill.attention(q, k, k, 0.1, causal=True, window=4)
+
+
+@pytest.mark.parametrize("n_q", [1, 32])
+def test_an_unaligned_workspace_is_refused_under_a_window(n_q):
+    a = _args(window=8, sinks=2, n_q=n_q, n_split=2)
+    a.workspace, a.workspace_bytes = (1 << 20) + 8, 1 << 20
+    assert _lib.lib().bmx_prefill(ct.byref(a), None) != 0
+    assert "16-byte" in _lib.lib().bmx_last_error().decode()
