@@ -16,9 +16,9 @@
 //                   top into the rows that grow (a stack place finds its row in
 //                   the prefix sums of grow).
 // A pool of up to kPgSmallPool ids and tables of up to kPgSmallCells entries take
-// one launch of one workgroup instead, the counts in its LDS (small_kernel): 8
-// beams of 512 pages over 8,192 ids 15.3 us against 17.0 of the four kernels, and
-// 20.3 us a call against 32.6 with their launches.
+// one launch of one workgroup instead, the counts and the stack in its LDS
+// (small_kernel): 8 beams of 512 pages over 8,192 ids 10.2 us against 14.7 of the
+// four kernels, and 20.4 us a call against 27.3 with their launches.
 //
 // compact, three launches: live pages a chunk; holes below n_live and movers
 // from there listed by rank; pages copied, entries and refs rewritten.
@@ -60,37 +60,46 @@ __device__ __forceinline__ int source_row(const UpdateArgs& a, int i) {
   return r >= 0 && r < a.rows ? r : -1;
 }
 
-// sum over the workgroup, in every thread
-__device__ __forceinline__ int block_sum(int v, int* s_tmp) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  __syncthreads();   // s_tmp may be in use by an earlier sum
-  if ((threadIdx.x & 63) == 0) s_tmp[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int t = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) t += s_tmp[w];
-  return t;
+// Sums over a workgroup are chains of latencies here (a launch has little else to
+// do): lanes add through DPP moves, not LDS, and the waves' sums are read at once.
+
+// inclusive prefix sum over the wave
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);    // row_shr:1 within 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+  return x;
 }
 
-// exclusive prefix sum over the workgroup's threads; total in every thread
-__device__ __forceinline__ int block_scan(int v, int* s_tmp, int& total) {
+// exclusive prefix sum over the workgroup's W waves; total in every thread
+template <int W>
+__device__ __forceinline__ int block_scan(int v, int (&s_tmp)[W], int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(x, o);
-    if (lane >= o) x += t;
-  }
-  __syncthreads();
+  const int x = wave_scan(v);
+  __syncthreads();   // s_tmp may be in use by an earlier sum
   if (lane == 63) s_tmp[wave] = x;
   __syncthreads();
-  int before = 0;
+  int before = 0, n[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) n[w] = s_tmp[w];
   total = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
-    if (w < wave) before += s_tmp[w];
-    total += s_tmp[w];
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    before += w < wave ? n[w] : 0;
+    total += n[w];
   }
   return before + x - v;
+}
+
+// sum over the workgroup, in every thread
+template <int W>
+__device__ __forceinline__ int block_sum(int v, int (&s_tmp)[W]) {
+  int total;
+  block_scan(v, s_tmp, total);
+  return total;
 }
 
 // workgroups 0 .. new_rows * pieces - 1: 1024 entries of a new row; then 1024 refs each
@@ -122,18 +131,20 @@ __global__ __launch_bounds__(kPgThreads) void count_kernel(const UpdateArgs a) {
   const int r = blockIdx.y;
   const int len = row_len(a.in, r, a.cap);
   if ((int)blockIdx.x * kPgChunk >= len) return;
+  int p[4];   // the row's pages, in flight during the count
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int e = (int)blockIdx.x * kPgChunk + threadIdx.x + u * kPgThreads;
+    p[u] = a.in.table[(int64_t)r * a.cap + min(e, len - 1)];
+    if (e >= len) p[u] = -1;
+  }
   int k = 0;
   for (int i = threadIdx.x; i < a.new_rows; i += kPgThreads) k += a.index[i] == r;
   k = block_sum(k, s_tmp) - 1;
   if (k == 0) return;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int e = (int)blockIdx.x * kPgChunk + threadIdx.x + u * kPgThreads;
-    if (e < len) {
-      const int p = a.in.table[(int64_t)r * a.cap + e];
-      if (p >= 0 && p < a.n_pool) atomicAdd(a.out.refs + p, k);
-    }
-  }
+  for (int u = 0; u < 4; ++u)
+    if (p[u] >= 0 && p[u] < a.n_pool) atomicAdd(a.out.refs + p[u], k);
 }
 
 __device__ __forceinline__ bool freed(const UpdateArgs& a, int p) { return a.in.refs[p] > 0 && a.out.refs[p] <= 0; }
@@ -166,6 +177,8 @@ __global__ __launch_bounds__(kPgThreads) void stack_kernel(const UpdateArgs a) {
     gone[u] = a.index && freed(a, p) && base + u < a.n_pool;
     id[u] = a.in.free[p];
   }
+  int len = tid < a.new_rows ? a.lens[tid] : 0, grow = tid < a.new_rows && a.grow ? max(a.grow[tid], 0) : 0;
+  const int n0 = min(max(*a.in.n_free, 0), a.n_pool);
   // freed pages before the chunk, and in all
   int before = 0, all = 0;
   if (a.index) {
@@ -177,23 +190,23 @@ __global__ __launch_bounds__(kPgThreads) void stack_kernel(const UpdateArgs a) {
     before = block_sum(before, s_tmp);
     all = block_sum(all, s_tmp);
   }
-  const int n0 = min(max(*a.in.n_free, 0), a.n_pool), top = min(n0 + all, a.n_pool);
+  const int top = min(n0 + all, a.n_pool);
   // what the rows ask for
   int64_t asked = 0;
   int wide = 0;
   for (int i0 = 0; i0 < a.new_rows; i0 += kPgThreads) {
     const int i = i0 + tid;
-    int g = 0;
-    if (i < a.new_rows) {
-      const int len = a.lens[i];
-      s_len[i] = len;
-      g = a.grow ? max(a.grow[i], 0) : 0;
-      wide |= g > a.cap - len;
-      g = min(g, a.n_pool + 1);   // a larger one fails the call by itself
+    if (i0 > 0) {
+      len = i < a.new_rows ? a.lens[i] : 0;
+      grow = i < a.new_rows && a.grow ? max(a.grow[i], 0) : 0;
     }
+    wide |= grow > a.cap - len;
     int sum;
-    const int at = block_scan(g, s_tmp, sum);
-    if (i < a.new_rows) s_first[i] = (int)min(asked + at, (int64_t)a.n_pool + 1);
+    const int at = block_scan(min(grow, a.n_pool + 1), s_tmp, sum);   // a larger one fails the call by itself
+    if (i < a.new_rows) {
+      s_len[i] = len;
+      s_first[i] = (int)min(asked + at, (int64_t)a.n_pool + 1);
+    }
     asked += sum;
   }
   wide = block_sum(wide, s_tmp);
@@ -243,111 +256,151 @@ __global__ __launch_bounds__(kPgThreads) void stack_kernel(const UpdateArgs a) {
 }
 
 constexpr int kPgSmallThreads = 1024;
-constexpr int kPgSmallPool = 16384;     // 64 KB of counts
-constexpr int kPgSmallRows = 1024;
+constexpr int kPgSmallPool = 16384;     // 64 KB of counts, as much of the stack
+constexpr int kPgSmallRows = kPgSmallThreads;
 constexpr int kPgSmallCells = 65536;    // entries of the old and new tables: a few us of one CU's traffic
 
-// An update by one workgroup: the passes of the four kernels over LDS counts.
+// LDS of small_kernel: refs, the new stack, which pages were live (a bit each), and
+// per row k (new rows that continue it), lengths, sources and first pages.
+__host__ __device__ __forceinline__ size_t small_lds(int n_pool, int rows, int new_rows) {
+  return 8 * (size_t)((n_pool + 63) / 64) + 4 * (2 * (size_t)n_pool + 2 * (size_t)rows + 3 * (size_t)new_rows);
+}
+
+// An update by one workgroup: the passes of the four kernels over LDS. Its time is
+// that of its chain of loads, LDS reads and barriers, so rows take 2^lg threads each
+// (no division), 4 rows are in flight, and rows are searched only for the pages given.
 __global__ __launch_bounds__(kPgSmallThreads) void small_kernel(const UpdateArgs a) {
-  extern __shared__ int s_mem[];
-  int* s_refs = s_mem;                       // [n_pool], then the freed ids are told from in.refs
-  int* s_k = s_refs + a.n_pool;              // [rows] new rows that continue the row
-  int* s_len = s_k + a.rows;                 // [new_rows]
+  constexpr int kWaves = kPgSmallThreads / 64, kU = 4;
+  extern __shared__ uint64_t s_live[];       // [n_pool / 64] in.refs > 0, then the freed ones
+  const int words = (a.n_pool + 63) / 64;
+  int* s_refs = reinterpret_cast<int*>(s_live + words);
+  int* s_stack = s_refs + a.n_pool;          // [n_pool]
+  int* s_k = s_stack + a.n_pool;             // [rows] new rows that continue the row
+  int* s_old = s_k + a.rows;                 // [rows] its pages
+  int* s_len = s_old + a.rows;               // [new_rows]
   int* s_first = s_len + a.new_rows;         // [new_rows]
-  __shared__ int s_tmp[kPgSmallThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = kPgSmallThreads / 64;
+  int* s_src = s_first + a.new_rows;         // [new_rows]
+  __shared__ int s_tmp[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per = (words + kWaves - 1) / kWaves, c0 = wave * per, c1 = min(c0 + per, words);   // the wave's ids, by 64
   const int n0 = min(max(*a.in.n_free, 0), a.n_pool);
-  for (int r = tid; r < a.rows; r += kPgSmallThreads) s_k[r] = 0;
-  for (int p = tid; p < a.n_pool; p += kPgSmallThreads) s_refs[p] = a.in.refs[p];
-  __syncthreads();
-  int64_t asked = 0;
-  int wide = 0;
-  for (int i0 = 0; i0 < a.new_rows; i0 += kPgSmallThreads) {
-    const int i = i0 + tid;
-    int g = 0;
-    if (i < a.new_rows) {
-      const int src = source_row(a, i), len = src < 0 ? 0 : row_len(a.in, src, a.cap);
-      if (src >= 0) atomicAdd(s_k + src, 1);
-      s_len[i] = len;
-      g = a.grow ? max(a.grow[i], 0) : 0;
-      wide |= g > a.cap - len;
-      g = min(g, a.n_pool + 1);
-    }
-    int sum;
-    const int at = block_scan(g, s_tmp, sum);
-    if (i < a.new_rows) s_first[i] = (int)min(asked + at, (int64_t)a.n_pool + 1);
-    asked += sum;
+  const int src = tid < a.new_rows ? source_row(a, tid) : -1;
+  const int grow = tid < a.new_rows && a.grow ? max(a.grow[tid], 0) : 0;
+  if (tid < a.rows) {
+    s_old[tid] = row_len(a.in, tid, a.cap);
+    s_k[tid] = 0;
   }
-  wide = block_sum(wide, s_tmp);   // and the rows' words are in LDS
-  // the tables, 64 entries a wave: an old row's pages lose or gain uses, a new row is its source's entries
-  const int pieces = (a.cap + 63) / 64;
-  if (a.index)
-    for (int t = wave; t < a.rows * pieces; t += waves) {
-      const int r = t / pieces, e = (t - r * pieces) * 64 + lane, k = s_k[r] - 1;
-      if (k != 0 && e < row_len(a.in, r, a.cap)) {
-        const int p = a.in.table[(int64_t)r * a.cap + e];
-        if (p >= 0 && p < a.n_pool) atomicAdd(s_refs + p, k);
+  for (int c = c0; c < c1; c += kU) {
+    int v[kU], f[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int p = min(64 * (c + u) + lane, a.n_pool - 1);
+      v[u] = a.in.refs[p];
+      f[u] = a.in.free[p];
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int p = 64 * (c + u) + lane;
+      const bool on = c + u < c1 && p < a.n_pool;
+      const uint64_t live = __ballot(on && v[u] > 0);
+      if (on) {
+        s_refs[p] = v[u];
+        s_stack[p] = p < n0 ? f[u] : -1;
       }
+      if (lane == 0 && c + u < c1) s_live[c + u] = live;
     }
-  for (int t = wave; t < a.new_rows * pieces; t += waves) {
-    const int i = t / pieces, e = (t - i * pieces) * 64 + lane, src = source_row(a, i);
-    if (e < a.cap) a.out.table[(int64_t)i * a.cap + e] = e < s_len[i] ? a.in.table[(int64_t)src * a.cap + e] : 0;
   }
   __syncthreads();
-  // freed ids, 64 a wave step: how many before the wave's, and in all
-  const int per = (a.n_pool + waves - 1) / waves, p0 = wave * per, p1 = min(p0 + per, a.n_pool);
-  auto is_freed = [&](int p) { return p < p1 && a.in.refs[p] > 0 && s_refs[p] <= 0; };
-  int mine = 0;
+  // new rows, one a thread
+  const int len = src < 0 ? 0 : s_old[src];
+  if (src >= 0) atomicAdd(s_k + src, 1);
+  int asked;
+  const int at = block_scan(min(grow, a.n_pool + 1), s_tmp, asked);   // a larger one fails the call by itself
+  if (tid < a.new_rows) {
+    s_len[tid] = len;
+    s_src[tid] = src;
+    s_first[tid] = min(at, a.n_pool + 1);
+  }
+  const bool wide = __syncthreads_or(tid < a.new_rows && grow > a.cap - len);   // and the rows' words are in LDS
+  // the tables: an old row's pages lose or gain uses, a new row is its source's entries
+  const int lg = min(10, 32 - __clz(a.cap - 1)), per_row = 1 << lg;   // >= cap, or all threads
+  const int r_first = tid >> lg, r_step = kPgSmallThreads >> lg, e_first = tid & (per_row - 1);
   if (a.index)
-    for (int p = p0 + lane; p < p0 + per; p += 64) mine += __popcll(__ballot(is_freed(p)));
-  mine = __builtin_amdgcn_readfirstlane(mine);
-  if (lane == 0) s_tmp[wave] = mine;
+    for (int r0 = r_first; r0 < a.rows; r0 += kU * r_step)
+      for (int e = e_first; e < a.cap; e += per_row) {
+        int p[kU], k[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int r = min(r0 + u * r_step, a.rows - 1);
+          k[u] = s_k[r] - 1;
+          p[u] = r0 + u * r_step < a.rows && k[u] != 0 && e < s_old[r] ? a.in.table[(int64_t)r * a.cap + e] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (p[u] >= 0 && p[u] < a.n_pool) atomicAdd(s_refs + p[u], k[u]);
+      }
+  for (int r0 = r_first; r0 < a.new_rows; r0 += kU * r_step)
+    for (int e = e_first; e < a.cap; e += per_row) {
+      int p[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int i = min(r0 + u * r_step, a.new_rows - 1);
+        p[u] = e < s_len[i] ? a.in.table[(int64_t)s_src[i] * a.cap + e] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (r0 + u * r_step < a.new_rows) a.out.table[(int64_t)(r0 + u * r_step) * a.cap + e] = p[u];
+    }
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < waves; ++w) {
-    before += w < wave ? s_tmp[w] : 0;
-    all += s_tmp[w];
+  // freed ids onto the stack, 64 a wave step: how many before the wave's, and in all
+  int top = n0;
+  if (a.index) {
+    int mine = 0;
+#pragma unroll 4
+    for (int c = c0; c < c1; ++c) {
+      const int p = 64 * c + lane;
+      const uint64_t m = s_live[c] & __ballot(p < a.n_pool && s_refs[p] <= 0);
+      mine += __popcll(m);
+      if (lane == 0) s_live[c] = m;
+    }
+    int all, j = n0 + block_scan(lane == 0 ? mine : 0, s_tmp, all);
+    j = __builtin_amdgcn_readfirstlane(j);
+    top = min(n0 + all, a.n_pool);
+#pragma unroll 4
+    for (int c = c0; c < c1; ++c) {
+      const uint64_t m = s_live[c];
+      const int place = j + __popcll(m & ((1ull << lane) - 1));
+      if ((m >> lane & 1) && place < a.n_pool) s_stack[place] = 64 * c + lane;
+      j += __popcll(m);
+    }
+    __syncthreads();
   }
-  const int top = min(n0 + all, a.n_pool);
-  const bool ok = wide == 0 && asked <= top;
-  const int given = ok ? (int)asked : 0, left = top - given;
-  auto place = [&](int j, int p) {   // as in stack_kernel
-    if (j >= top) return;
-    a.out.free[j] = j < left ? p : -1;
-    if (j < left) return;
-    const int k = top - 1 - j;
+  const bool ok = !wide && asked <= top;
+  const int given = ok ? asked : 0, left = top - given;
+  // the pages given: the k-th off the top to the last row whose pages begin at or before k
+  for (int k = tid; k < given; k += kPgSmallThreads) {
+    const int p = s_stack[top - 1 - k];
     int lo = 0, hi = a.new_rows - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (s_first[mid] <= k) lo = mid;
       else hi = mid - 1;
     }
-    const int at = s_len[lo] + k - s_first[lo];
-    if (at < a.cap) a.out.table[(int64_t)lo * a.cap + at] = p;
+    const int e = s_len[lo] + k - s_first[lo];
+    if (e < a.cap) a.out.table[(int64_t)lo * a.cap + e] = p;
     if (p >= 0 && p < a.n_pool) s_refs[p] = 1;
-  };
-  if (a.index) {
-    int j = n0 + before;
-    for (int p = p0 + lane; p < p0 + per; p += 64) {
-      const bool f = is_freed(p);
-      const uint64_t m = __ballot(f);
-      if (f) place(j + __popcll(m & ((1ull << lane) - 1)), p);
-      j += __popcll(m);
-    }
   }
-  __syncthreads();   // every freed id is told before a place of the old stack changes a count
-  for (int j = tid; j < a.n_pool; j += kPgSmallThreads) {
-    if (j < n0) place(j, a.in.free[j]);
-    else if (j >= top) a.out.free[j] = -1;
-  }
-  for (int i = tid; i < a.new_rows; i += kPgSmallThreads)
-    a.out.n_pages[i] = s_len[i] + (ok && a.grow ? max(a.grow[i], 0) : 0);
+  if (tid < a.new_rows) a.out.n_pages[tid] = len + (ok ? grow : 0);
   if (tid == 0) {
     *a.out.n_free = left;
     *a.status = wide ? BMX_PAGES_NO_ROOM : ok ? BMX_PAGES_OK : BMX_PAGES_NO_FREE;
   }
   __syncthreads();
-  for (int p = tid; p < a.n_pool; p += kPgSmallThreads) a.out.refs[p] = s_refs[p];
+#pragma unroll 4
+  for (int p = tid; p < a.n_pool; p += kPgSmallThreads) {
+    a.out.refs[p] = s_refs[p];
+    a.out.free[p] = p < left ? s_stack[p] : -1;
+  }
 }
 
 struct CompactArgs {
@@ -546,7 +599,7 @@ extern "C" int bmx_pages_update(const bmx_pages_update_args* a, void* stream) {
   const char* launched = "kernel launch: ";
   if (a->n_pool <= kPgSmallPool && a->rows <= kPgSmallRows && a->new_rows <= kPgSmallRows &&
       ((int64_t)a->rows + a->new_rows) * a->cap <= kPgSmallCells) {
-    const size_t lds = ((size_t)a->n_pool + a->rows + 2 * (size_t)a->new_rows) * sizeof(int);
+    const size_t lds = small_lds(a->n_pool, a->rows, a->new_rows);
     if (bmx_ensure_dynamic_lds((const void*)small_kernel, lds) != hipSuccess)
       return pg_fail(name, BMX_PAGES_E_HIP, "cannot reserve the kernel's LDS");
     hipLaunchKernelGGL(small_kernel, dim3(1), dim3(kPgSmallThreads), lds, st, k);
