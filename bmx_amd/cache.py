@@ -138,8 +138,9 @@ def packed_attention_forward(module, query, key, value, attention_mask, scaling,
         raise NotImplementedError("the packed cache serves batch size 1")
     q = query.squeeze(0)
     n_q = q.shape[1]
+    window = kwargs.get("sliding_window")   # layers that slide
     out = module._packed_layer.attend(q, scaling, is_causal=n_q > 1, attention_mask=attention_mask,
-                                      sliding_window=kwargs.get("sliding_window"))
+                                      **({"sliding_window": window} if window else {}))
     n_h, n_q, d = out.shape
     return out.transpose(0, 1).reshape(1, n_q, n_h * d).to(query.dtype), None
 
