@@ -18,10 +18,15 @@
 // A pool of up to kPgSmallPool ids and tables of up to kPgSmallCells entries take
 // one launch of one workgroup instead, the counts and the stack in its LDS
 // (small_kernel): 8 beams of 512 pages over 8,192 ids 10.2 us against 14.7 of the
-// four kernels, and 20.4 us a call against 27.3 with their launches.
+// four kernels, and 20.4 us a call against 27.3 with their launches.  At the limits
+// (32 rows of 512, 8,192 ids) 13.4 us against 11.8, the launches still ahead; past
+// them (64 rows of 512, 16,384 ids) 22.7 against 12.3.  64 rows of 4,096 pages over
+// 262,144 ids take the four 20 us.
 //
 // compact, three launches: live pages a chunk; holes below n_live and movers
-// from there listed by rank; pages copied, entries and refs rewritten.
+// from there listed by rank; pages copied, entries and refs rewritten.  A quarter
+// of 4,096 pages moved in the pools of 16 layers (376 MB read and written): 67 us in
+// move_kernel, 75 in all, 5.0 TB/s, the rate of a large copy.
 
 #include "bmx_pages.h"
 #include "k2b_common.h"
@@ -256,9 +261,9 @@ __global__ __launch_bounds__(kPgThreads) void stack_kernel(const UpdateArgs a) {
 }
 
 constexpr int kPgSmallThreads = 1024;
-constexpr int kPgSmallPool = 16384;     // 64 KB of counts, as much of the stack
+constexpr int kPgSmallPool = 8192;      // 32 KB of counts, as much of the stack
 constexpr int kPgSmallRows = kPgSmallThreads;
-constexpr int kPgSmallCells = 65536;    // entries of the old and new tables: a few us of one CU's traffic
+constexpr int kPgSmallCells = 32768;    // entries of the old and new tables: a few us of one CU's traffic
 
 // LDS of small_kernel: refs, the new stack, which pages were live (a bit each), and
 // per row k (new rows that continue it), lengths, sources and first pages.
