@@ -8,11 +8,10 @@
 // read.  With 4 rows a K/V element meets 16 flops, so the call is bound by its
 // bytes and, at the few MB of a window, by latency: the run is cut over the
 // chip so that a wave has all its loads in flight at once.  A window of 4,096 bf16
-// keys, 8 heads, G 4: 7.4 + 3.3 us (16.8 MB, 2.3 TB/s in the first kernel); 16 rows
-// over it 10.4 us, where 20 rows take 23.9 in the row tiles' form.
+// keys, 8 heads, G 4: 7.4 + 3.3 us (16.8 MB, 2.3 TB/s in the first kernel).
 //
-// rows_kernel<DT>: grid (splits, h_kv), 8 waves where one workgroup takes the
-// whole run (no merge), else 4.  A wave takes 64 tokens at a time (rows_step).
+// rows_kernel<DT>: grid (splits, h_kv, blocks of 16 rows), 8 waves where one
+// workgroup takes the whole run (no merge), else 4.  A wave takes 64 tokens at a time (rows_step).
 // The waves meet in LDS; one split writes the output, several write (sums, m, l)
 // partials that rows_merge_kernel joins.
 
@@ -25,6 +24,7 @@
 namespace bmx {
 namespace {
 
+constexpr int kRowsBlock = 16;      // rows of a workgroup: the columns of one 16x16 matrix product
 constexpr int kRwBatch = 64;        // tokens of a wave's step
 constexpr int kRwWaves = 4;         // waves of a workgroup, several splits
 constexpr int kRwWavesOne = 8;      // one split
@@ -46,8 +46,9 @@ struct RowsArgs {
 
 template <int DT>
 __global__ __launch_bounds__(64 * kRwWavesOne) void rows_kernel(const RowsArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float s_part[];   // [waves][R][kRwPitch]
+  extern __shared__ __attribute__((aligned(16))) float s_part[];   // [waves][n_rows][kRwPitch]
   const int split = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, waves = blockDim.x >> 6;
+  const int row0 = kRowsBlock * blockIdx.z, n_rows = min(kRowsBlock, a.R - row0);   // the workgroup's rows
   const int wave = tid >> 6, lane = tid & 63, q = lane >> 4, n = lane & 15;
   // the split's tokens in batches, dealt to the waves in turn
   const int n_batches = (a.T + kRwBatch - 1) / kRwBatch;
@@ -73,8 +74,8 @@ __global__ __launch_bounds__(64 * kRwWavesOne) void rows_kernel(const RowsArgs a
       for (int i = 0; i < 4; ++i)
         vr[j][i] = *reinterpret_cast<const u32x4_t*>(vh + (int64_t)key_of(v0 + 16 * j + 4 * q + i) * a.st + 8 * n);
   };
-  // the lane's row (rows past R repeat the last and are not stored)
-  const int row = min(n, a.R - 1), pos_i = row / a.G;
+  // the lane's row (lanes past the rows repeat the last and are not stored)
+  const int row = row0 + min(n, n_rows - 1), pos_i = row / a.G;
   const int last = a.p0 + pos_i, first = last - a.window + 1;
   u32x4_t qb[4];
   {
@@ -100,17 +101,17 @@ __global__ __launch_bounds__(64 * kRwWavesOne) void rows_kernel(const RowsArgs a
                   [&](int t) { return vh + (int64_t)key_of(v0 + t) * a.st; });
   }
   // ---- the waves meet in LDS
-  rows_store(st, n < a.R, s_part + (wave * a.R + n) * kRwPitch);
+  rows_store(st, n < n_rows, s_part + (wave * n_rows + n) * kRwPitch);
   __syncthreads();
-  for (int e = tid; e < a.R * (kRwD / 4); e += blockDim.x) {
+  for (int e = tid; e < n_rows * (kRwD / 4); e += blockDim.x) {
     const int x = e >> 5, c = 4 * (e & 31);
     const float* src = s_part + x * kRwPitch;
     float M = -INFINITY;
-    for (int w = 0; w < waves; ++w) M = fmaxf(M, src[w * a.R * kRwPitch + kRwD]);
+    for (int w = 0; w < waves; ++w) M = fmaxf(M, src[w * n_rows * kRwPitch + kRwD]);
     float den = 0.f;
     float4_t num = {0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < waves; ++w) {
-      const float* ws = src + w * a.R * kRwPitch;
+      const float* ws = src + w * n_rows * kRwPitch;
       const float2 ml = *reinterpret_cast<const float2*>(ws + kRwD);
       const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
       den = __builtin_fmaf(f, ml.y, den);
@@ -118,11 +119,11 @@ __global__ __launch_bounds__(64 * kRwWavesOne) void rows_kernel(const RowsArgs a
     }
     if (a.n_split == 1) {
       const float inv = den == 0.f ? 0.f : 1.0f / den;
-      const int i = x / a.G, g = x - i * a.G;
+      const int i = (row0 + x) / a.G, g = row0 + x - i * a.G;
       *reinterpret_cast<uint2*>(a.out + ((int64_t)(h * a.G + g) * a.n_q + i) * kRwD + c) =
           make_uint2(rw_pack2<DT>(num[0] * inv, num[1] * inv), rw_pack2<DT>(num[2] * inv, num[3] * inv));
     } else {
-      float* po = a.part + (((int64_t)h * a.R + x) * a.n_split + split) * kRwPitch;
+      float* po = a.part + (((int64_t)h * a.R + row0 + x) * a.n_split + split) * kRwPitch;
       *reinterpret_cast<float4_t*>(po + c) = num;
       if (c == 0) *reinterpret_cast<float2*>(po + kRwD) = make_float2(M, den);
     }
@@ -206,11 +207,12 @@ RowsArgs rows_run(const bmx_prefill_args* a) {
 // workgroups of 4 waves, up to 16 of 2 steps (2,000 keys 8.3 us, of 4 steps 9.2),
 // more of 4 steps (4,096 keys 9.0 us, of 2 steps 9.8; 32,000 keys of one head 11.9
 // and 14.3), as long as that is no more than 4 workgroups a CU.
+int row_blocks(const bmx_prefill_args* a) { return (a->n_q * a->n_q_groups + kRowsBlock - 1) / kRowsBlock; }
 int rows_splits(const bmx_prefill_args* a, int T) {
   if (a->n_split > 0) return a->n_split;
   const int batches = (T + kRwBatch - 1) / kRwBatch;
   if (batches <= kRwWavesOne) return 1;
-  const int most = std::max(1, 4 * bmx_device_cu_count() / a->h_kv);
+  const int most = std::max(1, 4 * bmx_device_cu_count() / (a->h_kv * row_blocks(a)));
   const int splits = std::max((batches + kRwWaves - 1) / kRwWaves, std::min(16, (batches + 1) / 2));
   return std::max(1, std::min(splits, most));
 }
@@ -237,8 +239,8 @@ hipError_t rows_launch(const bmx_prefill_args* a, hipStream_t st) {
   k.n_split = rows_splits(a, k.T);
   k.qscale = a->sm_scale * 1.4426950408889634f;
   const int waves = k.n_split == 1 ? kRwWavesOne : kRwWaves;
-  const size_t lds = (size_t)waves * k.R * kRwPitch * sizeof(float);
-  const dim3 grid((unsigned)k.n_split, (unsigned)a->h_kv), rows((unsigned)k.R, (unsigned)a->h_kv);
+  const size_t lds = (size_t)waves * std::min(k.R, kRowsBlock) * kRwPitch * sizeof(float);
+  const dim3 grid((unsigned)k.n_split, (unsigned)a->h_kv, (unsigned)row_blocks(a)), rows((unsigned)k.R, (unsigned)a->h_kv);
   const bool f16 = a->dtype == BMX_PREFILL_F16;
   auto launch = [&](auto kernel) {
     const hipError_t e = bmx_ensure_dynamic_lds((const void*)kernel, lds);

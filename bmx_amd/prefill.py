@@ -49,8 +49,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *
     ``window`` > 0 as well only those with ``j > p - window`` (HF's
     sliding_window: the query's own key is one of the window) or ``j < sinks``.
     Under a window, rows that a query does not see may hold anything (infinities
-    and NaN among it) and do not reach its output.  Few rows (n_q * G up to 16, a
-    token's attention) under a window run on a form of their own, the keys
+    and NaN among it) and do not reach its output.  Few rows (n_q * G up to 64, a
+    token's attention or a few drafted ones) under a window run on a form of their own, the keys
     spread over the chip.
     Returns (h_kv * G, n_q, 128) in q's dtype, contiguous."""
     _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape, "q (Hq, n_q, 128), k and v (h_kv, n_kv, 128)")

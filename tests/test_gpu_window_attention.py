@@ -108,6 +108,38 @@ def test_window_attention_matches_64_bits(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [
+    # several blocks of 16 rows: h_kv, G, n_q, n_kv, window, sinks, n_split
+    (2, 4, 5, 6000, 700, 4, 0), (1, 7, 9, 1000, 130, 20, 0), (2, 1, 33, 500, 40, 0, 1), (1, 1, 64, 64, 1, 0, 0),
+    (3, 16, 4, 900, 300, 4, 5), (1, 64, 1, 4000, 2000, 1, 0), (1, 3, 21, 21, 8, 2, 16), (1, 5, 13, 300, 50, 4, 0),
+    (2, 2, 32, 9000, 100000, 4, 0),
+])
+def test_blocks_of_rows_match_64_bits(case, dtype):
+    h_kv, G, n_q, n_kv, window, sinks, n_split = case
+    print(f"row blocks {case} {dtype}", flush=True)
+    q, k, v = _inputs(h_kv, G, n_q, n_kv, dtype, seed=n_q * 5 + n_kv)
+    out = prefill.attention(q, k, v, SCALE, causal=True, window=window, sinks=sinks, n_split=n_split)
+    torch.cuda.synchronize()
+    _check(out, q, k, v, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_hidden_infinity_stays_out_of_every_block_of_rows(dtype):
+    """48 rows of one head over 3 blocks: a value that only the middle ones see."""
+    n_q, n_kv, window = 48, 400, 16
+    q, k, v = _inputs(1, 1, n_q, n_kv, dtype, seed=9)
+    at = n_kv - n_q + 10
+    clean = prefill.attention(q, k, v, SCALE, causal=True, window=window)
+    v[0, at, 5] = float("-inf")
+    out = prefill.attention(q, k, v, SCALE, causal=True, window=window)
+    torch.cuda.synchronize()
+    sees = _seen(n_q, n_kv, window, 0)[:, at]
+    assert sees.sum() == window
+    assert torch.equal(out[0, ~sees], clean[0, ~sees])
+    assert not torch.isfinite(out[0, sees][:, 5]).any() and torch.isfinite(out[0, sees][:, 6:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n_q,G", [(150, 4), (1, 4), (3, 2)])
 def test_strided_operands_and_peaked_scores(n_q, G, dtype):
     """q as a projection's transposed view, K/V rows inside a longer buffer
