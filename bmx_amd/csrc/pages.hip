@@ -361,7 +361,6 @@ __global__ __launch_bounds__(kPgSmallThreads) void small_kernel(const UpdateArgs
   int top = n0;
   if (a.index) {
     int mine = 0;
-#pragma unroll 4
     for (int c = c0; c < c1; ++c) {
       const int p = 64 * c + lane;
       const uint64_t m = s_live[c] & __ballot(p < a.n_pool && s_refs[p] <= 0);
